@@ -350,6 +350,90 @@ int tsb_norm_gemv_bf16(const float* x_in, const float* delta, float* x_out, cons
 int tsb_gemv_bf16_residual(const void* weight, const void* bias, int32_t N, int32_t K, const void* x, float* resid,
                            const float* norm_weight, float eps, void* h_out, uint32_t* counter, void* stream);
 
+/* ---- paged KV cache, attention over it, and token sampling ---------------
+ * The operators of a serving step whose requests share one pool of cache
+ * pages (tinyserve/paged_kv_cache.py:20-122), with the sliding window that
+ * keeps the first tokens visible of tinyserve/static_kv_cache.py:282-389.
+ *
+ * TsbPagedCache: pools of keys and values.  Element (page, head, row, d) of
+ *   either is at page * page_stride + head * head_stride + row * row_stride +
+ *   d (elements; strides multiples of 16 bytes, base pointers 16-byte
+ *   aligned), so [pages, heads, rows, D] and [pages, rows, heads, D] both
+ *   work.  They hold `dtype` (TSB_DT_BF16 / TSB_DT_F16), or e4m3 when
+ *   cache_fp8 is set.  head_dim 64 or 128; any page_size >= 1.
+ * TsbPagedBatch: a ragged batch.  Sequence b's new tokens are the rows
+ *   [cu_q[b], cu_q[b+1]) of the call's n_tokens rows and the last of the
+ *   kv_lens[b] positions it holds with them; position j is row j % page_size
+ *   of page page_table[b * table_stride + j / page_size].  cu_q (ascending,
+ *   n_seqs + 1 entries), kv_lens and page_table are on the device; max_q is an
+ *   upper bound of the new tokens of any sequence.  Rows that belong to no
+ *   sequence are not written.  Entries that contradict this (a page outside
+ *   the pool, a length beyond the table) are reported as device error
+ *   2 and never dereferenced. */
+typedef struct {
+  void* k_cache;
+  void* v_cache;
+  int64_t page_stride, head_stride, row_stride; /* elements, the same for keys and values */
+  int32_t num_pages, page_size, n_kv_heads, head_dim;
+  int32_t dtype;     /* type of qkv, q and out; of the caches too unless cache_fp8 */
+  int32_t cache_fp8; /* 1: the caches hold e4m3 */
+} TsbPagedCache;
+
+typedef struct {
+  const int32_t* page_table;
+  const int32_t* cu_q;
+  const int32_t* kv_lens;
+  int32_t table_stride, table_width; /* entries between rows of the table, entries used per row */
+  int32_t n_seqs, n_tokens, max_q;
+} TsbPagedBatch;
+
+/* Workspace of the two paged entry points, 256-byte aligned, zero-initialised
+ * once; one workspace serves successive calls on a stream (any batch).
+ * tsb_read_device_error(workspace, ...) reads its error word. */
+size_t tsb_paged_workspace(int32_t head_dim);
+
+/* RoPE and cache store of a fused projection's rows: qkv [n_tokens,
+ * (n_q_heads + 2 n_kv_heads) * head_dim], rows qkv_stride elements apart; cos
+ * / sin [max_pos, head_dim / 2] (table_dtype TSB_DT_F32 or the cache's dtype),
+ * halves rotated, the angle of a token's position.  The rotated queries go to
+ * q_out [n_tokens, n_q_heads, head_dim]; rotated keys and the values are
+ * rounded to dtype and stored in their pages (e4m3: rounded once more, values
+ * beyond its range become NaN as a plain cast makes them). */
+int tsb_paged_kv_store(const TsbPagedCache* cache, const TsbPagedBatch* batch, const void* qkv, int64_t qkv_stride,
+                       int32_t n_q_heads, const void* cos, const void* sin, int32_t table_dtype, int32_t max_pos,
+                       void* q_out, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Attention of the batch's new tokens over the pages.  The token at position
+ * p sees j <= p and, with window > 0, only j > p - window or j < keep_first.
+ * Softmax over scale * q.k in fp32 with the head's sink logit sinks[n_q_heads]
+ * in the denominator (NULL: none); a row that sees nothing gives zeros.
+ * q [n_tokens, n_q_heads, head_dim] with the given strides (elements, multiples
+ * of 8; 16-byte aligned), out contiguous, both of the cache's dtype. */
+int tsb_paged_attention(const TsbPagedCache* cache, const TsbPagedBatch* batch, const void* q, int64_t q_token_stride,
+                        int64_t q_head_stride, int32_t n_q_heads, int32_t window, int32_t keep_first,
+                        const float* sinks, float scale, void* out, void* workspace, size_t workspace_bytes,
+                        void* stream);
+
+/* One token per row of logits [rows, vocab] (dtype TSB_DT_*, rows row_stride
+ * elements apart).  Tokens are ranked by (logit descending, index ascending);
+ * with w_i = exp((x_i - max) / temperature) a row keeps its first top_k
+ * (<= 0 or >= vocab: all), of these the shortest prefix whose mass reaches
+ * top_p of theirs (>= 1: all), of these the tokens with w >= min_p (<= 0:
+ * all), and always the first.  It draws the kept token with the largest
+ * (x_i - max) / temperature - log(noise_i); with exponential variates in
+ * noise [rows, vocab] (noise_stride apart) that is a draw from the kept
+ * distribution.  A row with temperature <= 0 takes its first token (and counts
+ * as temperature 1 in logprobs), and so does every row when noise is NULL.
+ * temperature, top_k, top_p, min_p: per row, each may be NULL (1, all, all,
+ * all).
+ * logprobs[row] (or NULL) = (x - max) / temperature - log(sum_i w_i) of the
+ * drawn token, over the whole row.  NaN logits count as -infinity; a row of
+ * nothing else gives token -1 and log-probability -infinity; with +infinity
+ * logits only those are drawn. */
+int tsb_sample(const void* logits, int32_t dtype, int32_t rows, int32_t vocab, int64_t row_stride, const float* noise,
+               int64_t noise_stride, const float* temperature, const int32_t* top_k, const float* top_p,
+               const float* min_p, int64_t* tokens, float* logprobs, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

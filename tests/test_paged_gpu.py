@@ -1,0 +1,384 @@
+"""Paged KV store and paged attention against their definitions in 64 bits, at
+the lengths, masks, page sizes and layouts where they can go wrong."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from tests import paged_reference as R
+
+pytestmark = pytest.mark.gpu
+
+BF, F16, E4 = torch.bfloat16, torch.float16, torch.float8_e4m3fn
+# half an ulp of the 16-bit types, relative: bf16 has 8 significant bits, f16 has 11
+HALF_ULP = {BF: 2.0 ** -8, F16: 2.0 ** -11}
+
+
+@pytest.fixture(scope="module")
+def ops():
+    if not torch.cuda.is_available():
+        pytest.skip("CUDA required")
+    from tinyserve_b200 import ops
+    return ops
+
+
+def attend(ops, b, **kw):
+    sinks = b.sinks if kw.pop("sinks", True) else None
+    return ops.paged_attention(b.q, b.k, b.v, b.table, b.cu, b.kv, b.max_q, sinks=sinks, **kw)
+
+
+def check(got, b, **kw):
+    """Weights and the output are each rounded once to a 16-bit type (half an
+    ulp u of |out| and of the magnitude sum w |v|); scores are fp32 sums of up
+    to 128 products of size below 32 (error below 2^-13 each, so 2^-12 of the
+    magnitude after exp, and the sums of weights); f16 also has its smallest
+    step."""
+    ref, mag = R.attention(b, **kw)
+    u = HALF_ULP[b.dtype]
+    got = got.double().cpu().numpy()
+    bound = u * np.abs(ref) + (u + 2.0 ** -12) * mag + 2.0 ** -24
+    assert np.isfinite(got).all()
+    worst = np.max(np.abs(got - ref) / bound) if got.size else 0.0
+    assert worst <= 1.0, f"{worst:.2f} times the bound"
+
+
+# new tokens and cached positions: single tokens, a first prompt, chunks that end inside a page or a tile,
+# an idle slot, more new tokens than positions (rows that see nothing)
+RAGGED = ([1, 1, 0, 7, 33, 1, 5, 130], [1, 300, 0, 7, 100, 129, 3, 150])
+SINGLE = ([1] * 6, [1, 2, 64, 65, 511, 1000])
+SHORT = ([2, 3, 1, 2], [2, 40, 17, 260])
+PROMPT = ([257, 1, 16], [257, 16, 16])
+
+
+@pytest.mark.parametrize("held", ["same", "e4m3"])
+@pytest.mark.parametrize("dtype", [BF, F16])
+@pytest.mark.parametrize("d,heads", [(64, (8, 1)), (64, (4, 4)), (128, (6, 2)), (128, (16, 1)), (64, (14, 2))])
+@pytest.mark.parametrize("lens", [RAGGED, SINGLE, SHORT, PROMPT], ids=["ragged", "single", "short", "prompt"])
+def test_attention(ops, lens, d, heads, dtype, held):
+    b = R.Batch(*lens, *heads, d, 16, dtype, E4 if held == "e4m3" else dtype, seed=d + heads[0])
+    check(attend(ops, b), b)
+
+
+@pytest.mark.parametrize("page", [1, 8, 24, 100, 256])
+@pytest.mark.parametrize("lens", [RAGGED, SINGLE], ids=["ragged", "single"])
+def test_page_sizes(ops, page, lens):
+    b = R.Batch(*lens, 8, 2, 64, page, BF, BF, seed=page)
+    check(attend(ops, b), b)
+
+
+@pytest.mark.parametrize("held", [BF, E4])
+@pytest.mark.parametrize("sinks", [True, False])
+@pytest.mark.parametrize("window,keep", [(1, 0), (1, 3), (37, 0), (37, 4), (128, 1), (128, 140), (5000, 4)])
+def test_window_and_first_tokens(ops, window, keep, sinks, held):
+    for lens in (RAGGED, ([1, 1, 3, 1], [900, 129, 500, 20]), ([200], [640])):
+        b = R.Batch(*lens, 8, 2, 64, 16, BF, held, seed=window + keep)
+        kw = dict(window=window, keep_first=keep, sinks=sinks)
+        check(attend(ops, b, **kw), b, **kw)
+
+
+def test_long_contexts_are_split(ops):
+    """Few rows over many positions: the key range is divided and joined."""
+    for lens in (([1], [20011]), ([3, 1], [9000, 12345]), ([40], [6001])):
+        b = R.Batch(*lens, 8, 1, 64, 64, BF, E4, seed=5)
+        check(attend(ops, b), b)
+
+
+def test_rows_that_see_nothing_are_zero(ops):
+    b = R.Batch([4, 20], [0, 2], 8, 2, 64, 16, BF, BF)
+    for sinks in (True, False):
+        out = attend(ops, b, sinks=sinks)
+        assert (out[:4] == 0).all() and (out[4:22] == 0).all() and (out[22:] != 0).any()
+        check(out, b, sinks=sinks)
+
+
+@pytest.mark.parametrize("held", [BF, E4])
+@pytest.mark.parametrize("q,kv", [(40, 300), (2, 70), (1, 90)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_what_the_mask_hides_does_not_matter(ops, bad, q, kv, held):
+    """NaN and infinities in keys and values that a row may not see: later
+    tokens of its chunk, positions before its window, page tails and unused
+    pages (filled with NaN by the batch).  The rows that do see them are NaN or
+    infinite, and only those."""
+    if held == E4 and bad == float("inf"):
+        bad = float("nan")  # e4m3 has no infinity
+    b = R.Batch([q], [kv], 8, 2, 64, 16, BF, held, seed=q)
+    window, keep = 30, 2
+    clean = attend(ops, b, window=window, keep_first=keep)
+    check(clean, b, window=window, keep_first=keep)
+    late, early = kv - 1 - q // 2, max(keep, kv - q - window)  # seen by the later rows; by no row
+    for pool in (b.k, b.v):
+        for j in {early} | ({late + 1} if q > 1 else set()):
+            page, row = int(b.table[0, j // 16]), j % 16
+            pool[page, :, row] = torch.tensor(bad).to(held)
+    out = attend(ops, b, window=window, keep_first=keep)
+    p = torch.arange(kv - q, kv, device="cuda")
+    hit = torch.zeros(q, dtype=torch.bool, device="cuda")
+    for j in {early} | ({late + 1} if q > 1 else set()):
+        hit |= (j <= p) & ((j > p - window) | (j < keep))
+    assert torch.equal(out[~hit], clean[~hit])
+    assert not torch.isfinite(out[hit]).any()
+
+
+def test_values_alone_hidden_by_the_mask(ops):
+    """Only a value is not finite: its row of V meets a weight of zero."""
+    for q, kv in ((50, 50), (200, 333), (2, 40)):
+        b = R.Batch([q], [kv], 8, 1, 64, 16, BF, BF, seed=kv)
+        clean = attend(ops, b)
+        j = kv - 1
+        b.v[int(b.table[0, j // 16]), :, j % 16, 5] = float("inf")
+        out = attend(ops, b)
+        assert torch.equal(out[:-1], clean[:-1])
+        assert torch.equal(out[-1, :, :5], clean[-1, :, :5]) and torch.equal(out[-1, :, 6:], clean[-1, :, 6:])
+        assert (out[-1, :, 5] == float("inf")).all()
+
+
+@pytest.mark.parametrize("held", [BF, E4])
+def test_layouts_and_strides(ops, held):
+    """Pools stored by rows, q as a view of the fused projection, padding rows."""
+    for lens in (RAGGED, SINGLE):
+        b = R.Batch(*lens, 8, 2, 64, 16, BF, held, layout="rows")
+        assert not b.k.is_contiguous()
+        qkv = torch.randn(b.n + 5, 12, 64, device="cuda").to(BF)
+        qkv[:b.n, :8] = b.q
+        out = torch.full((b.n + 5, 8, 64), 7.0, dtype=BF, device="cuda")
+        ops.paged_attention(qkv[:, :8], b.k, b.v, b.table, b.cu, b.kv, b.max_q, sinks=b.sinks, out=out)
+        check(out[:b.n], b)
+        assert (out[b.n:] == 7.0).all()  # rows of no sequence
+
+
+def test_large_scores_and_scales(ops):
+    """One key far above the rest at either end, a negative and a zero scale."""
+    for lens in (([1, 3], [400, 300]), ([150], [400])):
+        b = R.Batch(*lens, 8, 1, 64, 16, BF, BF, seed=9)
+        for j in (0, 255, 299):
+            b.k[int(b.table[0, j // 16]), :, j % 16] *= 16
+        for scale in (1.0, -0.125, 0.0):
+            ref, mag = R.attention(b, scale=scale)
+            got = attend(ops, b, scale=scale).double().cpu().numpy()
+            # scores reach 16 * 64 * 20 * scale: fp32 sums of 64 products err by 2^-18 of that size
+            err = 2.0 ** -12 + 2 * 64 * 20 * 20 * abs(scale) * 2.0 ** -18
+            assert (np.abs(got - ref) <= HALF_ULP[BF] * np.abs(ref) + (HALF_ULP[BF] + err) * mag + 1e-30).all()
+
+
+def test_wide_range_of_q(ops):
+    """q of either end of bf16's range over an 8-bit cache, and tiny ones."""
+    for size in (1e-30, 1e-6, 3e4, 1e30):
+        for lens in (([1], [100]), ([40], [100])):
+            b = R.Batch(*lens, 8, 1, 64, 16, BF, E4, seed=3)
+            b.q = (b.q.float() * size).to(BF)
+            check(attend(ops, b, scale=0.125 / size), b, scale=0.125 / size)
+
+
+def test_offsets_beyond_32_bits(ops):
+    """Pages that start past 2^32 elements of the pool."""
+    b = R.Batch([1, 40], [100, 60], 8, 1, 64, 16, BF, E4, seed=1)
+    far = (1 << 32) // 1024 + 7
+    for name in ("k", "v"):
+        small = getattr(b, name)
+        big = torch.empty(far + small.shape[0], 1, 16, 64, dtype=E4, device="cuda")
+        big[far:] = small
+        setattr(b, name, big)
+    b.table[b.table >= 0] += far
+    out = attend(ops, b)
+    b.k, b.v, b.table = b.k[far:], b.v[far:], torch.where(b.table >= 0, b.table - far, b.table)
+    check(out, b)
+
+
+def test_same_result_every_time_and_on_another_stream(ops):
+    for lens in (([1, 1], [5000, 77]), RAGGED):
+        b = R.Batch(*lens, 8, 2, 64, 16, BF, BF)
+        first = attend(ops, b)
+        for _ in range(3):
+            assert torch.equal(attend(ops, b), first)
+        st = torch.cuda.Stream()
+        st.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(st):
+            out = attend(ops, b)
+        st.synchronize()
+        assert torch.equal(out, first)
+
+
+def test_in_a_graph(ops):
+    """Captured once, replayed with other lengths and tables in place."""
+    b = R.Batch([1, 1, 20], [300, 900, 50], 8, 2, 64, 16, BF, BF, seed=1)
+    other = R.Batch([1, 1, 20], [800, 5, 200], 8, 2, 64, 16, BF, BF, seed=2, spare=0)
+    pool = max(b.k.shape[0], other.k.shape[0])
+    for t in (b, other):
+        for n in ("k", "v"):
+            grown = torch.zeros(pool, 2, 16, 64, dtype=BF, device="cuda")
+            grown[:getattr(t, n).shape[0]] = getattr(t, n)
+            setattr(t, n, grown)
+        table = torch.full((3, 64), -1, dtype=torch.int32, device="cuda")
+        table[:, :t.table.shape[1]] = t.table
+        t.table = table
+    st = torch.cuda.Stream()
+    with torch.cuda.stream(st):
+        attend(ops, b)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=st):
+            out = attend(ops, b)
+        g.replay()
+        st.synchronize()
+        check(out, b)
+        for n in ("k", "v", "q", "kv", "table", "sinks"):
+            getattr(b, n).copy_(getattr(other, n))
+        g.replay()
+        st.synchronize()
+    check(out, other)
+
+
+@pytest.mark.parametrize("held", ["same", "e4m3"])
+@pytest.mark.parametrize("tables", ["same", "f32"])
+@pytest.mark.parametrize("dtype", [BF, F16])
+@pytest.mark.parametrize("d", [64, 128])
+def test_store(ops, d, dtype, tables, held):
+    """Rotated q and k within one rounding of the 64-bit product (and three of
+    fp32), what is stored exactly that rounded value (e4m3: rounded once
+    more), nothing else of the pools touched."""
+    nq, nkv = 6, 2
+    b = R.Batch(RAGGED[0], [max(q, k) for q, k in zip(*RAGGED)], nq, nkv, d, 24, dtype, E4 if held == "e4m3" else dtype,
+                fill=0.25)
+    g = torch.Generator().manual_seed(d)
+    wide = torch.randn(b.n, (nq + 2 * nkv) * d + 16, generator=g).to(dtype).cuda()
+    qkv = wide[:, :(nq + 2 * nkv) * d]
+    ang = torch.arange(400)[:, None] * 10000.0 ** (-torch.arange(0, d, 2) / d)[None, :]
+    cos, sin = (t.to(torch.float32 if tables == "f32" else dtype).cuda() for t in (ang.cos(), ang.sin()))
+    k0, v0 = b.k.clone(), b.v.clone()
+    q = ops.paged_kv_store(qkv, cos, sin, b.k, b.v, b.table, b.cu, b.kv, n_q_heads=nq)
+    x = qkv.double().view(b.n, nq + 2 * nkv, d)
+    pos = torch.cat([torch.arange(k - n, k) for n, k in zip(b.q_lens, b.kv_lens)]).cuda()
+    seq = torch.cat([torch.full((n,), i) for i, n in enumerate(b.q_lens)]).cuda()
+    c, s = cos.double()[pos][:, None], sin.double()[pos][:, None]
+    lo, hi = x[..., :d // 2], x[..., d // 2:]
+    ref = torch.cat([lo * c - hi * s, hi * c + lo * s], -1)
+    size = torch.cat([(lo * c).abs() + (hi * s).abs(), (hi * c).abs() + (lo * s).abs()], -1)
+    u = HALF_ULP[dtype]
+
+    def near(got, want, m):
+        assert ((got.double() - want).abs() <= u * want.abs() + 2.0 ** -22 * m + 2.0 ** -25).all()
+
+    near(q, ref[:, :nq], size[:, :nq])
+    cf, sf, lf, hf = c.float(), s.float(), lo.float()[:, :nq], hi.float()[:, :nq]
+    assert torch.equal(q, torch.cat([lf * cf - hf * sf, hf * cf + lf * sf], -1).to(dtype))  # one rounding each
+    page, row = b.table[seq, pos // 24].long(), pos % 24
+    if held == "same":
+        near(b.k[page, :, row], ref[:, nq:nq + nkv], size[:, nq:nq + nkv])
+        assert torch.equal(b.v[page, :, row], qkv.reshape(b.n, nq + 2 * nkv, d)[:, nq + nkv:])
+    else:
+        # the 16-bit value a 16-bit cache gets, rounded once more
+        k16, v16 = torch.zeros_like(b.k, dtype=dtype), torch.zeros_like(b.v, dtype=dtype)
+        ops.paged_kv_store(qkv, cos, sin, k16, v16, b.table, b.cu, b.kv, n_q_heads=nq)
+        for pool, pool16 in ((b.k, k16), (b.v, v16)):
+            assert torch.equal(pool.view(torch.uint8)[page, :, row], pool16[page, :, row].to(E4).view(torch.uint8))
+    untouched = torch.ones(b.k.shape[0], 24, dtype=torch.bool, device="cuda")
+    untouched[page, row] = False
+    for pool, before in ((b.k, k0), (b.v, v0)):
+        keep = untouched[:, None, :, None].expand_as(pool)
+        assert torch.equal(pool.float()[keep], before.float()[keep])
+
+
+def test_store_then_attend(ops):
+    """A prompt in chunks through both operators equals it in one go."""
+    nq, nkv, d, n = 8, 2, 64, 150
+    g = torch.Generator().manual_seed(4)
+    qkv = torch.randn(n, (nq + 2 * nkv) * d, generator=g).to(BF).cuda()
+    ang = torch.arange(n)[:, None] * 10000.0 ** (-torch.arange(0, d, 2) / d)[None, :]
+    cos, sin = ang.cos().cuda(), ang.sin().cuda()
+
+    def through(cuts):
+        k = torch.zeros(12, nkv, 16, d, dtype=BF, device="cuda")
+        v = torch.zeros_like(k)
+        table = torch.arange(11, -1, -1, dtype=torch.int32, device="cuda")[None]
+        outs, at = [], 0
+        for c in cuts:
+            cu = torch.tensor([0, c], dtype=torch.int32, device="cuda")
+            kv = torch.tensor([at + c], dtype=torch.int32, device="cuda")
+            q = ops.paged_kv_store(qkv[at:at + c], cos, sin, k, v, table, cu, kv, n_q_heads=nq)
+            outs.append(ops.paged_attention(q, k, v, table, cu, kv, c, window=60, keep_first=3))
+            at += c
+        return torch.cat(outs), k, v
+
+    whole, k1, v1 = through([n])
+    parts, k2, v2 = through([64, 1, 1, 33, 51])
+    assert torch.equal(k1, k2) and torch.equal(v1, v2)
+    # both hold the bound of one rounding of the weights and one of the output
+    assert ((whole.float() - parts.float()).abs() <= 4 * HALF_ULP[BF] * (whole.float().abs() + v1.float().abs().max())).all()
+
+
+def test_inconsistent_batches_are_reported_not_read(ops):
+    """A page outside the pool, a length beyond the table, a cu_q that runs past
+    the rows or above max_q: device error 2, and the sound sequences are served."""
+    good = R.Batch([1, 2, 40], [50, 60, 70], 8, 2, 64, 16, BF, BF)
+    want = attend(ops, good)
+    assert ops.paged_device_error() == 0
+    for what in ("page", "length", "rows", "max_q"):
+        b = R.Batch([1, 2, 40], [50, 60, 70], 8, 2, 64, 16, BF, BF)
+        if what == "page":
+            b.table[2, 1] = b.k.shape[0]
+        elif what == "length":
+            b.kv[2] = 16 * b.table.shape[1] + 1
+        elif what == "rows":
+            b.cu[3] += 1
+        else:
+            b.max_q = 39
+        out = attend(ops, b)
+        assert torch.equal(out[:3], want[:3]), what
+        assert ops.paged_device_error() == 2, what
+        assert ops.paged_device_error() == 0
+    b = R.Batch([4], [50], 8, 2, 64, 16, BF, BF)
+    qkv = torch.zeros(4, 12 * 64, dtype=BF, device="cuda")
+    t = torch.zeros(48, 32, device="cuda")  # two positions short
+    k0 = b.k.clone()
+    b.table[0, 2] = -5
+    ops.paged_kv_store(qkv, t, t, b.k, b.v, b.table, b.cu, b.kv, n_q_heads=8)
+    assert ops.paged_device_error() == 2
+    changed = (b.k.view(torch.int16) != k0.view(torch.int16)).any(-1).any(1)  # [page, row]
+    assert changed.sum() == 0  # 46 and 47 fall in the missing page, 48 and 49 past the tables
+
+
+def test_empty_calls(ops):
+    b = R.Batch([0, 0], [5, 0], 8, 2, 64, 16, BF, BF)
+    assert attend(ops, b).shape == (0, 8, 64)
+    b = R.Batch([], [], 8, 2, 64, 16, BF, BF)
+    assert attend(ops, b).shape == (0, 8, 64)
+    qkv = torch.zeros(0, 12 * 64, dtype=BF, device="cuda")
+    t = torch.zeros(4, 32, device="cuda")
+    assert ops.paged_kv_store(qkv, t, t, b.k, b.v, b.table, b.cu, b.kv, n_q_heads=8).shape == (0, 8, 64)
+
+
+def test_refusals(ops):
+    b = R.Batch([1], [5], 8, 2, 64, 16, BF, BF)
+
+    def call(**kw):
+        a = dict(q=b.q, k=b.k, v=b.v, table=b.table, cu=b.cu, kv=b.kv, max_q=1, sinks=b.sinks) | kw
+        more = {n: a.pop(n) for n in list(a) if n not in ("q", "k", "v", "table", "cu", "kv", "max_q")}
+        return ops.paged_attention(*a.values(), **more)
+
+    for error, kw in (
+            (RuntimeError, dict(q=b.q.cpu())), (TypeError, dict(q=b.q.float())), (TypeError, dict(q=b.q.half())),
+            (ValueError, dict(q=b.q[0])), (ValueError, dict(q=b.q[..., :32])),
+            (ValueError, dict(v=b.v[:, :1])), (ValueError, dict(v=b.v.transpose(1, 2).contiguous().transpose(1, 2))),
+            (ValueError, dict(k=b.k.transpose(2, 3), v=b.v.transpose(2, 3))),
+            (ValueError, dict(table=b.table.long())), (ValueError, dict(table=b.table[0])),
+            (ValueError, dict(cu=b.cu.long())), (ValueError, dict(cu=b.cu[:1])), (ValueError, dict(kv=b.kv.long())),
+            (ValueError, dict(sinks=b.sinks.double())), (ValueError, dict(sinks=b.sinks[:4])),
+            (ValueError, dict(out=torch.empty(1, 8, 64, device="cuda"))),
+            (RuntimeError, dict(window=-1)), (RuntimeError, dict(keep_first=-1)), (RuntimeError, dict(max_q=-1)),
+            (RuntimeError, dict(q=b.q.repeat(1, 2, 1)[:, :9], sinks=None)),
+            (RuntimeError, dict(workspace=torch.zeros(16, dtype=torch.uint8, device="cuda"))),
+            (RuntimeError, dict(k=b.k[..., :32].contiguous(), v=b.v[..., :32].contiguous(),
+                                q=b.q[..., :32].contiguous()))):
+        with pytest.raises(error):
+            call(**kw)
+    odd = torch.zeros(64 * 16 * 2 * 8 + 1, dtype=BF, device="cuda")[1:].view(8, 2, 16, 64)
+    with pytest.raises(RuntimeError, match="aligned"):
+        call(k=odd, v=odd)
+    t = torch.zeros(8, 32, device="cuda")
+    qkv = torch.zeros(1, 12 * 64, dtype=BF, device="cuda")
+    for kw in (dict(cos=t[:, :16]), dict(cos=t.double(), sin=t.double()), dict(qkv=qkv[:, :64]),
+               dict(q_out=torch.empty(1, 8, 64, device="cuda"))):
+        a = dict(qkv=qkv, cos=t, sin=t) | kw
+        more = {"q_out": a.pop("q_out")} if "q_out" in a else {}
+        with pytest.raises(ValueError):
+            ops.paged_kv_store(a["qkv"], a["cos"], a["sin"], b.k, b.v, b.table, b.cu, b.kv, n_q_heads=8, **more)

@@ -35,6 +35,7 @@ EXPORTS = (
     "tsb_ep_moe_prefill", "tsb_gqa_decode_workspace", "tsb_gqa_decode_attention", "tsb_add_rmsnorm",
     "tsb_gemv_bf16", "tsb_norm_gemv_bf16", "tsb_gemv_bf16_residual", "tsb_gqa_decode_batch_workspace",
     "tsb_gqa_decode_attention_batch", "tsb_norm_qkv_attention",
+    "tsb_paged_workspace", "tsb_paged_kv_store", "tsb_paged_attention", "tsb_sample",
 )
 
 
@@ -54,6 +55,24 @@ class TsbExpert(ctypes.Structure):
         ("gate", ctypes.c_void_p), ("up", ctypes.c_void_p), ("down", ctypes.c_void_p),
         ("gate_scales", ctypes.c_void_p), ("up_scales", ctypes.c_void_p), ("down_scales", ctypes.c_void_p),
         ("gate_bias", ctypes.c_void_p), ("up_bias", ctypes.c_void_p), ("down_bias", ctypes.c_void_p),
+    ]
+
+
+class TsbPagedCache(ctypes.Structure):
+    _fields_ = [
+        ("k_cache", ctypes.c_void_p), ("v_cache", ctypes.c_void_p),
+        ("page_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64), ("row_stride", ctypes.c_int64),
+        ("num_pages", ctypes.c_int32), ("page_size", ctypes.c_int32),
+        ("n_kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+        ("dtype", ctypes.c_int32), ("cache_fp8", ctypes.c_int32),
+    ]
+
+
+class TsbPagedBatch(ctypes.Structure):
+    _fields_ = [
+        ("page_table", ctypes.c_void_p), ("cu_q", ctypes.c_void_p), ("kv_lens", ctypes.c_void_p),
+        ("table_stride", ctypes.c_int32), ("table_width", ctypes.c_int32),
+        ("n_seqs", ctypes.c_int32), ("n_tokens", ctypes.c_int32), ("max_q", ctypes.c_int32),
     ]
 
 
@@ -105,6 +124,13 @@ def _declare(L: ctypes.CDLL) -> None:
     L.tsb_norm_gemv_bf16.argtypes = [_vp, _vp, _vp, _vp, ctypes.c_float, _vp, _vp, _i32, _i32, _vp, _vp]
     L.tsb_gemv_bf16_residual.argtypes = [_vp, _vp, _i32, _i32, _vp, _vp, _vp, ctypes.c_float, _vp, _vp, _vp]
     L.tsb_add_rmsnorm.argtypes = [_vp, _vp, _i32, _vp, ctypes.c_float, _i32, _i32, _vp, _vp]
+    pc, pb = ctypes.POINTER(TsbPagedCache), ctypes.POINTER(TsbPagedBatch)
+    L.tsb_paged_workspace.argtypes = [_i32]
+    L.tsb_paged_workspace.restype = _sz
+    L.tsb_paged_kv_store.argtypes = [pc, pb, _vp, _i64, _i32, _vp, _vp, _i32, _i32, _vp, _vp, _sz, _vp]
+    L.tsb_paged_attention.argtypes = [pc, pb, _vp, _i64, _i64, _i32, _i32, _i32, _vp, ctypes.c_float, _vp, _vp, _sz,
+                                      _vp]
+    L.tsb_sample.argtypes = [_vp, _i32, _i32, _i32, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp]
     L.tsb_ep_prefill_workspace.argtypes = [ctypes.POINTER(TsbMoeSpec), _i32, _i32]
     L.tsb_ep_prefill_workspace.restype = _sz
     L.tsb_ep_moe_prefill.argtypes = [ctypes.POINTER(TsbMoeSpec), _vp, _vp, _i32, _vp, _vp, _vp, _vp, _i32, _i32, _vp,

@@ -1,0 +1,353 @@
+// RoPE + store into a paged KV cache, and attention of a ragged batch of new
+// tokens over it (tsb_paged_kv_store, tsb_paged_attention).
+//
+// The cache is a pool of pages shared by all requests
+// (tinyserve/paged_kv_cache.py:20-122); a sliding window may keep the first
+// tokens visible (tinyserve/static_kv_cache.py:282-389); GPT-OSS adds a sink
+// logit per head to the softmax denominator.
+//
+//   out_t = sum_j e^(s_tj - m) v_j / (e^(sink - m) + sum_j e^(s_tj - m)),
+//   s_tj = scale * q_t . k_j,  j visible to t,  m the running maximum.
+#include <type_traits>
+
+#include "paged.cuh"
+
+namespace tsb {
+namespace {
+
+// ------------------------------------------------------------------ store
+// One CTA per token; a thread takes 8 dims of a head's lower half with the 8
+// of its upper half (two 16-byte loads, two 16-byte stores), so rotation
+// needs no exchange.  Products and sums are rounded one by one in fp32 (no
+// contraction), then once to the 16-bit type.
+struct StoreArgs {
+  PagedArgs p;
+  const uint16_t* qkv;
+  int64_t qkv_stride;
+  const void* cos;
+  const void* sin;
+  uint16_t* q_out;
+  int max_rope;
+};
+
+template <int DT, bool TF32>
+__device__ __forceinline__ void load_table8(const void* t, int64_t at, float (&r)[8]) {
+  if constexpr (TF32) {
+    const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(t) + at);
+    const float4 a = p[0], b = p[1];
+    r[0] = a.x, r[1] = a.y, r[2] = a.z, r[3] = a.w;
+    r[4] = b.x, r[5] = b.y, r[6] = b.z, r[7] = b.w;
+  } else {
+    const uint4 v = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(t) + at);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      r[2 * i] = to_f32<DT>((uint16_t)w[i]);
+      r[2 * i + 1] = to_f32<DT>((uint16_t)(w[i] >> 16));
+    }
+  }
+}
+
+template <int DT>
+__device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    w[i] = (uint32_t)from_f32<DT>(x[2 * i]) | ((uint32_t)from_f32<DT>(x[2 * i + 1]) << 16);
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// 8 values of the 16-bit type, rounded once more to e4m3.
+template <int DT>
+__device__ __forceinline__ uint2 pack8_e4m3(uint4 v) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  uint32_t o[2] = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float f = to_f32<DT>((uint16_t)(w[i / 2] >> (16 * (i & 1))));
+    o[i / 4] |= (uint32_t)__nv_cvt_float_to_fp8(f, __NV_NOSAT, __NV_E4M3) << (8 * (i & 3));
+  }
+  return make_uint2(o[0], o[1]);
+}
+
+template <int DT, int D, bool FP8, bool TF32>
+__global__ void __launch_bounds__(256) paged_store_kernel(const StoreArgs s) {
+  const PagedArgs& a = s.p;
+  constexpr int kC = D / 16;  // 8-dim chunks of a half
+  const int token = blockIdx.x;
+  const int b = seq_of(a, token);
+  if (b < 0) return;
+  const SeqSpan sp = seq_span(a, b);
+  const int pos = sp.kv_len - sp.q_len + (token - sp.q0);
+  if (token - sp.q0 >= sp.q_len) return;  // a span that was reported and cut
+  if (pos < 0 || pos >= s.max_rope) {
+    if (threadIdx.x == 0) atomicExch(a.err, kDevBadPlan);
+    return;
+  }
+  const int64_t row = cached_row(a, b, pos);
+  const uint16_t* src = s.qkv + (int64_t)token * s.qkv_stride;
+  for (int u = threadIdx.x; u < (a.nq + 2 * a.nkv) * kC; u += blockDim.x) {
+    const int head = u / kC, c = u - head * kC;
+    const uint4 r1 = *reinterpret_cast<const uint4*>(src + head * D + c * 8);
+    const uint4 r2 = *reinterpret_cast<const uint4*>(src + head * D + D / 2 + c * 8);
+    uint4 o1 = r1, o2 = r2;
+    if (head < a.nq + a.nkv) {
+      float cs[8], sn[8], y1[8], y2[8];
+      load_table8<DT, TF32>(s.cos, (int64_t)pos * (D / 2) + c * 8, cs);
+      load_table8<DT, TF32>(s.sin, (int64_t)pos * (D / 2) + c * 8, sn);
+      const uint32_t w1[4] = {r1.x, r1.y, r1.z, r1.w}, w2[4] = {r2.x, r2.y, r2.z, r2.w};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float x1 = to_f32<DT>((uint16_t)(w1[i / 2] >> (16 * (i & 1))));
+        const float x2 = to_f32<DT>((uint16_t)(w2[i / 2] >> (16 * (i & 1))));
+        y1[i] = __fsub_rn(__fmul_rn(x1, cs[i]), __fmul_rn(x2, sn[i]));
+        y2[i] = __fadd_rn(__fmul_rn(x2, cs[i]), __fmul_rn(x1, sn[i]));
+      }
+      o1 = pack8<DT>(y1);
+      o2 = pack8<DT>(y2);
+    }
+    if (head < a.nq) {
+      uint16_t* q = s.q_out + ((int64_t)token * a.nq + head) * D;
+      *reinterpret_cast<uint4*>(q + c * 8) = o1;
+      *reinterpret_cast<uint4*>(q + D / 2 + c * 8) = o2;
+    } else if (row >= 0) {
+      const bool key = head < a.nq + a.nkv;
+      const int64_t at = row + (int64_t)(head - a.nq - (key ? 0 : a.nkv)) * a.head_stride + c * 8;
+      uint8_t* pool = const_cast<uint8_t*>(key ? a.kc : a.vc);
+      if constexpr (FP8) {
+        *reinterpret_cast<uint2*>(pool + at) = pack8_e4m3<DT>(o1);
+        *reinterpret_cast<uint2*>(pool + at + D / 2) = pack8_e4m3<DT>(o2);
+      } else {
+        *reinterpret_cast<uint4*>(pool + 2 * at) = o1;
+        *reinterpret_cast<uint4*>(pool + 2 * (at + D / 2)) = o2;
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------ attention
+struct AttnCall {
+  PagedArgs p;
+  const uint16_t* q;
+  uint16_t* out;
+  int64_t q_token_stride, q_head_stride;
+  const float* sinks;
+  float scale;
+  int window, keep_first;
+};
+
+// One warp per (token, head): the lanes split the head's dimensions, the keys
+// are walked one by one with a running maximum and sum.
+template <int DT, int D, bool FP8>
+__global__ void __launch_bounds__(256) paged_attn_rows(const AttnCall c) {
+  const PagedArgs& a = c.p;
+  constexpr int E = D / 32;
+  const int lane = threadIdx.x & 31;
+  const int64_t w = (int64_t)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
+  if (w >= (int64_t)a.n_tokens * a.nq) return;
+  const int token = (int)(w / a.nq), head = (int)(w % a.nq);
+  const int b = seq_of(a, token);
+  if (b < 0) return;
+  const SeqSpan sp = seq_span(a, b);
+  if (token - sp.q0 >= sp.q_len) return;
+  const int pos = sp.kv_len - sp.q_len + (token - sp.q0);
+  const uint16_t* q = c.q + token * c.q_token_stride + head * c.q_head_stride + lane * E;
+  float qv[E], o[E] = {};
+#pragma unroll
+  for (int e = 0; e < E; ++e) qv[e] = to_f32<DT>(q[e]) * c.scale;
+  float m = -INFINITY, l = 0.f;
+  const int low = c.window > 0 ? max(0, pos - c.window + 1) : 0;
+  for (int j = 0; j <= pos; ++j) {
+    if (j == min(c.keep_first, low)) j = low;  // the gap between the first tokens and the window
+    const int64_t row = cached_row(a, b, j);
+    if (row < 0) continue;
+    const int64_t at = row + (int64_t)(head / a.G) * a.head_stride + lane * E;
+    float s = 0.f, v[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      float k;
+      if constexpr (FP8) {
+        k = e4m3_to_f32(a.kc[at + e]);
+        v[e] = e4m3_to_f32(a.vc[at + e]);
+      } else {
+        k = to_f32<DT>(reinterpret_cast<const uint16_t*>(a.kc)[at + e]);
+        v[e] = to_f32<DT>(reinterpret_cast<const uint16_t*>(a.vc)[at + e]);
+      }
+      s = fmaf(qv[e], k, s);
+    }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+    const float mn = fmaxf(m, s), base = mn == -INFINITY ? 0.f : mn;
+    const float keep = expf(m - base), p = expf(s - base);
+    l = l * keep + p;
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = fmaf(p, v[e], o[e] * keep);
+    m = mn;
+  }
+  if (c.sinks) {
+    const float sink = c.sinks[head], mn = fmaxf(m, sink), base = mn == -INFINITY ? 0.f : mn, keep = expf(m - base);
+    l = l * keep + expf(sink - base);
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] *= keep;
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  uint16_t* out = c.out + ((int64_t)token * a.nq + head) * D + lane * E;
+#pragma unroll
+  for (int e = 0; e < E; ++e) out[e] = from_f32<DT>(o[e] * inv);
+}
+
+// ------------------------------------------------------------------ host
+int fail(int code, const char* what) { return set_error(code, what); }
+
+// Checks what both entry points share and fills the kernel's arguments.
+int paged_args(const TsbPagedCache* c, const TsbPagedBatch* b, int n_q_heads, void* ws, size_t ws_bytes, PagedArgs& a) {
+  if (!c || !b || !ws) return fail(TSB_ERR_INVALID, "null pointer");
+  if (c->head_dim != 64 && c->head_dim != 128) return fail(TSB_ERR_UNSUPPORTED, "head_dim must be 64 or 128");
+  if (c->dtype != TSB_DT_BF16 && c->dtype != TSB_DT_F16) return fail(TSB_ERR_UNSUPPORTED, "dtype must be bf16 or f16");
+  if (c->cache_fp8 != 0 && c->cache_fp8 != 1) return fail(TSB_ERR_INVALID, "cache_fp8 must be 0 or 1");
+  if (c->n_kv_heads <= 0 || n_q_heads <= 0 || n_q_heads % c->n_kv_heads)
+    return fail(TSB_ERR_INVALID, "n_q_heads must be a positive multiple of n_kv_heads");
+  if (c->num_pages < 0 || c->page_size <= 0) return fail(TSB_ERR_INVALID, "page_size must be positive");
+  if (b->n_seqs < 0 || b->n_tokens < 0 || b->max_q < 0 || b->table_width < 0 || b->table_stride < b->table_width)
+    return fail(TSB_ERR_INVALID, "bad batch sizes");
+  if ((int64_t)b->table_width * c->page_size > INT32_MAX / 2) return fail(TSB_ERR_UNSUPPORTED, "page table too wide");
+  if ((int64_t)b->n_tokens * n_q_heads > INT32_MAX / 2) return fail(TSB_ERR_UNSUPPORTED, "too many tokens in one call");
+  const int64_t per16 = c->cache_fp8 ? 16 : 8;
+  if (c->page_stride % per16 || c->head_stride % per16 || c->row_stride % per16 || c->page_stride < 0 ||
+      c->head_stride < 0 || c->row_stride < 0)
+    return fail(TSB_ERR_INVALID, "cache strides must be multiples of 16 bytes");
+  if ((reinterpret_cast<uintptr_t>(c->k_cache) | reinterpret_cast<uintptr_t>(c->v_cache)) & 15)
+    return fail(TSB_ERR_INVALID, "caches must be 16-byte aligned");
+  if (b->n_tokens > 0 && b->n_seqs > 0 &&
+      (!c->k_cache || !c->v_cache || !b->cu_q || !b->kv_lens || (b->table_width > 0 && !b->page_table)))
+    return fail(TSB_ERR_INVALID, "null pointer");
+  if (reinterpret_cast<uintptr_t>(ws) & 255) return fail(TSB_ERR_INVALID, "workspace must be 256-byte aligned");
+  if (ws_bytes < tsb_paged_workspace(c->head_dim)) return fail(TSB_ERR_WORKSPACE, "workspace too small");
+  a.kc = static_cast<const uint8_t*>(c->k_cache);
+  a.vc = static_cast<const uint8_t*>(c->v_cache);
+  a.page_stride = c->page_stride;
+  a.head_stride = c->head_stride;
+  a.row_stride = c->row_stride;
+  a.table = b->page_table;
+  a.cu_q = b->cu_q;
+  a.kv_lens = b->kv_lens;
+  a.err = static_cast<int32_t*>(ws);
+  a.num_pages = c->num_pages;
+  a.page_size = c->page_size;
+  a.table_stride = b->table_stride;
+  a.max_pos = b->table_width * c->page_size;
+  a.n_seqs = b->n_seqs;
+  a.n_tokens = b->n_tokens;
+  a.max_q = b->max_q;
+  a.nq = n_q_heads;
+  a.nkv = c->n_kv_heads;
+  a.G = n_q_heads / c->n_kv_heads;
+  return TSB_OK;
+}
+
+// Calls f with the cache's type, head size and storage as constants.
+template <class F>
+void dispatch_paged(const TsbPagedCache& c, F f) {
+  auto by_type = [&](auto dt, auto d) {
+    if (c.cache_fp8)
+      f(dt, d, std::true_type{});
+    else
+      f(dt, d, std::false_type{});
+  };
+  auto by_dim = [&](auto dt) {
+    if (c.head_dim == 64)
+      by_type(dt, std::integral_constant<int, 64>{});
+    else
+      by_type(dt, std::integral_constant<int, 128>{});
+  };
+  if (c.dtype == TSB_DT_BF16)
+    by_dim(std::integral_constant<int, TSB_DT_BF16>{});
+  else
+    by_dim(std::integral_constant<int, TSB_DT_F16>{});
+}
+
+int launched() {
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? TSB_OK : fail(TSB_ERR_CUDA, cudaGetErrorString(e));
+}
+
+}  // namespace
+}  // namespace tsb
+
+using namespace tsb;
+
+extern "C" {
+
+size_t tsb_paged_workspace(int32_t head_dim) {
+  if (head_dim != 64 && head_dim != 128) return 0;
+  return kPagedHead;
+}
+
+int tsb_paged_kv_store(const TsbPagedCache* cache, const TsbPagedBatch* batch, const void* qkv, int64_t qkv_stride,
+                       int32_t n_q_heads, const void* cos, const void* sin, int32_t table_dtype, int32_t max_pos,
+                       void* q_out, void* workspace, size_t workspace_bytes, void* stream) {
+  StoreArgs s{};
+  const int rc = paged_args(cache, batch, n_q_heads, workspace, workspace_bytes, s.p);
+  if (rc) return rc;
+  if (table_dtype != TSB_DT_F32 && table_dtype != cache->dtype)
+    return fail(TSB_ERR_UNSUPPORTED, "cos / sin must be fp32 or the cache's dtype");
+  if (batch->n_tokens == 0 || batch->n_seqs == 0) return TSB_OK;
+  if (!qkv || !cos || !sin || !q_out) return fail(TSB_ERR_INVALID, "null pointer");
+  if (qkv_stride < (int64_t)(n_q_heads + 2 * cache->n_kv_heads) * cache->head_dim || qkv_stride % 8)
+    return fail(TSB_ERR_INVALID, "qkv rows must not overlap and be a multiple of 8 elements apart");
+  if ((reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(cos) | reinterpret_cast<uintptr_t>(sin) |
+       reinterpret_cast<uintptr_t>(q_out)) & 15)
+    return fail(TSB_ERR_INVALID, "qkv, cos, sin and q_out must be 16-byte aligned");
+  s.qkv = static_cast<const uint16_t*>(qkv);
+  s.qkv_stride = qkv_stride;
+  s.cos = cos;
+  s.sin = sin;
+  s.q_out = static_cast<uint16_t*>(q_out);
+  s.max_rope = max_pos;
+  const dim3 grid(batch->n_tokens);
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  auto go = [&](auto dt, auto d, auto fp8, auto tf) {
+    paged_store_kernel<decltype(dt)::value, decltype(d)::value, decltype(fp8)::value, decltype(tf)::value>
+        <<<grid, 256, 0, st>>>(s);
+  };
+  dispatch_paged(*cache, [&](auto dt, auto d, auto fp8) {
+    if (table_dtype == TSB_DT_F32)
+      go(dt, d, fp8, std::true_type{});
+    else
+      go(dt, d, fp8, std::false_type{});
+  });
+  return launched();
+}
+
+int tsb_paged_attention(const TsbPagedCache* cache, const TsbPagedBatch* batch, const void* q, int64_t q_token_stride,
+                        int64_t q_head_stride, int32_t n_q_heads, int32_t window, int32_t keep_first,
+                        const float* sinks, float scale, void* out, void* workspace, size_t workspace_bytes,
+                        void* stream) {
+  AttnCall c{};
+  const int rc = paged_args(cache, batch, n_q_heads, workspace, workspace_bytes, c.p);
+  if (rc) return rc;
+  if (window < 0 || keep_first < 0) return fail(TSB_ERR_INVALID, "window and keep_first must not be negative");
+  if (batch->n_tokens == 0 || batch->n_seqs == 0) return TSB_OK;
+  if (!q || !out) return fail(TSB_ERR_INVALID, "null pointer");
+  if (q_token_stride % 8 || q_head_stride % 8 || q_token_stride < 0 || q_head_stride < 0)
+    return fail(TSB_ERR_INVALID, "q strides must be multiples of 8 elements");
+  if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15)
+    return fail(TSB_ERR_INVALID, "q and out must be 16-byte aligned");
+  c.q = static_cast<const uint16_t*>(q);
+  c.out = static_cast<uint16_t*>(out);
+  c.q_token_stride = q_token_stride;
+  c.q_head_stride = q_head_stride;
+  c.sinks = sinks;
+  c.scale = scale;
+  c.window = window;
+  c.keep_first = window > 0 ? keep_first : 0;
+  const int64_t rows = (int64_t)batch->n_tokens * n_q_heads;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  dispatch_paged(*cache, [&](auto dt, auto d, auto fp8) {
+    paged_attn_rows<decltype(dt)::value, decltype(d)::value, decltype(fp8)::value>
+        <<<(unsigned)((rows + 7) / 8), 256, 0, st>>>(c);
+  });
+  return launched();
+}
+
+}  // extern "C"

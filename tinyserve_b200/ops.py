@@ -68,6 +68,191 @@ def weight_bytes(fmt: int, rows: int, cols: int) -> tuple[int, int]:
 
 
 # ---------------------------------------------------------------------------
+# A paged KV cache, attention over it and token sampling: the operators of a
+# serving step (tinyserve/paged_kv_cache.py:20-122; sliding window with
+# visible first tokens, tinyserve/static_kv_cache.py:282-389).
+# ---------------------------------------------------------------------------
+_paged_ws: dict[tuple[int, int, int], torch.Tensor] = {}
+
+
+def paged_workspace(device: torch.device, head_dim: int) -> torch.Tensor:
+    """Zero-initialised scratch of the paged operators.  One workspace serves
+    successive calls on one stream; the operators keep one per (device,
+    stream) unless they are given another."""
+    return torch.zeros(_lib.lib().tsb_paged_workspace(head_dim), dtype=torch.uint8, device=device)
+
+
+def _paged_workspace(device: torch.device, head_dim: int, stream: int) -> torch.Tensor:
+    key = (device.index, head_dim, stream)
+    ws = _paged_ws.get(key)
+    if ws is None:
+        ws = _paged_ws[key] = paged_workspace(device, head_dim)
+    return ws
+
+
+def paged_device_error(workspace: torch.Tensor | None = None, device: torch.device | None = None) -> int:
+    """Read and clear the device error word of a workspace, or of every
+    workspace the paged operators keep for ``device``: 0 when the batches were
+    consistent, 2 when one named a page outside the pool or a length beyond
+    its table.  Synchronises."""
+    if workspace is None:
+        device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+        held = [ws for key, ws in _paged_ws.items() if key[0] == (device.index or 0)]
+    else:
+        held = [workspace]
+    code = 0
+    for ws in held:
+        torch.cuda.synchronize(ws.device)
+        c = ctypes.c_int32()
+        _lib.check(_lib.lib().tsb_read_device_error(ws.data_ptr(), ctypes.byref(c), _stream(ws.device)))
+        code = code or c.value
+    return code
+
+
+def _paged_call(rows: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
+                cu_q: torch.Tensor, kv_lens: torch.Tensor, max_q: int):
+    """The C structs of a paged call (kept alive by the caller), after the
+    checks that need the tensors themselves."""
+    if not (rows.is_cuda and k_cache.is_cuda and v_cache.is_cuda and page_table.is_cuda and cu_q.is_cuda
+            and kv_lens.is_cuda):
+        raise RuntimeError("tinyserve_b200 kernels need CUDA tensors")
+    dtype = rows.dtype
+    if dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError("tokens must be bfloat16 or float16")
+    if k_cache.dtype not in (dtype, torch.float8_e4m3fn):
+        raise TypeError("the cache must hold the tokens' dtype or float8_e4m3fn")
+    ks = k_cache.stride()
+    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or ks != v_cache.stride() or v_cache.dtype != k_cache.dtype:
+        raise ValueError("k_cache and v_cache must be alike: [pages, kv_heads, page_size, head_dim]")
+    if ks[3] != 1:
+        raise ValueError("the caches' last dimension must be contiguous")
+    n_seqs = page_table.shape[0]
+    if page_table.dim() != 2 or page_table.dtype != torch.int32 or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+        raise ValueError("page_table must be int32 [sequences, pages] with contiguous rows")
+    if (cu_q.dtype != torch.int32 or kv_lens.dtype != torch.int32 or cu_q.dim() != 1 or kv_lens.dim() != 1
+            or cu_q.numel() != n_seqs + 1 or kv_lens.numel() != n_seqs or not cu_q.is_contiguous()
+            or not kv_lens.is_contiguous()):
+        raise ValueError("cu_q and kv_lens must be contiguous int32 of sequences + 1 and sequences entries")
+    pages, nkv, page, d = k_cache.shape
+    width = page_table.shape[1]
+    cache = _lib.TsbPagedCache(k_cache.data_ptr(), v_cache.data_ptr(), ks[0], ks[1], ks[2], pages, page, nkv, d,
+                               _DT[dtype], 1 if k_cache.element_size() == 1 else 0)
+    batch = _lib.TsbPagedBatch(page_table.data_ptr(), cu_q.data_ptr(), kv_lens.data_ptr(),
+                               max(width, page_table.stride(0) if n_seqs > 1 else width), width, n_seqs,
+                               rows.shape[0], max_q)
+    return cache, batch
+
+
+def paged_kv_store(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_cache: torch.Tensor,
+                   v_cache: torch.Tensor, page_table: torch.Tensor, cu_q: torch.Tensor, kv_lens: torch.Tensor, *,
+                   n_q_heads: int, q_out: torch.Tensor | None = None,
+                   workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Rotate a fused projection's queries and keys and put keys and values into
+    their pages; returns the rotated queries [N, n_q_heads, D].
+
+    qkv         [N, (n_q_heads + 2 kv_heads) * D] bf16 / f16, contiguous rows: the new tokens of all sequences
+    cos, sin    [positions, D / 2] fp32 or qkv's dtype; halves rotated (the GPT-OSS convention)
+    k_cache, v_cache  [pages, kv_heads, page_size, D] of qkv's dtype or float8_e4m3fn, any strides with a
+                contiguous last dimension; D 64 or 128
+    page_table  int32 [B, pages per sequence]
+    cu_q        int32 [B + 1]: rows of sequence b are cu_q[b] .. cu_q[b + 1] - 1
+    kv_lens     int32 [B]: positions held once the new tokens are in; those are its last ones
+    """
+    n, d = qkv.shape[0], k_cache.shape[-1]
+    cache, batch = _paged_call(qkv, k_cache, v_cache, page_table, cu_q, kv_lens, n)
+    if qkv.dim() != 2 or qkv.shape[1] != (n_q_heads + 2 * cache.n_kv_heads) * d or (n and qkv.stride(1) != 1):
+        raise ValueError("qkv must be [tokens, (n_q_heads + 2 kv_heads) * head_dim] with contiguous rows")
+    if (cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != sin.dtype or cos.shape[1] * 2 != d
+            or cos.dtype not in (torch.float32, qkv.dtype) or not cos.is_contiguous() or not sin.is_contiguous()):
+        raise ValueError("cos and sin must be contiguous [positions, head_dim / 2] of fp32 or qkv's dtype")
+    _require_cuda(cos, sin, q_out)
+    if q_out is None:
+        q_out = torch.empty(n, n_q_heads, d, dtype=qkv.dtype, device=qkv.device)
+    elif q_out.shape != (n, n_q_heads, d) or q_out.dtype != qkv.dtype or not q_out.is_contiguous():
+        raise ValueError("q_out must be contiguous [tokens, n_q_heads, head_dim] of qkv's dtype")
+    stream = _stream(qkv.device)
+    ws = _paged_workspace(qkv.device, d, stream) if workspace is None else workspace
+    _lib.check(_lib.lib().tsb_paged_kv_store(
+        ctypes.byref(cache), ctypes.byref(batch), qkv.data_ptr(), max(qkv.stride(0), qkv.shape[1]), n_q_heads,
+        cos.data_ptr(), sin.data_ptr(), _DT[cos.dtype], cos.shape[0], q_out.data_ptr(), ws.data_ptr(), ws.numel(),
+        stream))
+    return q_out
+
+
+def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
+                    cu_q: torch.Tensor, kv_lens: torch.Tensor, max_q: int, *, scale: float | None = None,
+                    window: int = 0, keep_first: int = 0, sinks: torch.Tensor | None = None,
+                    out: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal attention of a ragged batch of new tokens (prompt chunks and
+    single decode tokens together) over the pages; [N, n_q_heads, D].
+
+    q           [N, n_q_heads, D] bf16 / f16, last dimension contiguous
+    max_q       upper bound of the new tokens of any sequence
+    window      0: every earlier position; else the last ``window`` positions and the first ``keep_first``
+    sinks       fp32 [n_q_heads]: a logit per head that joins the softmax denominator only
+    The other arguments are paged_kv_store's.  A token that sees nothing gives zeros.
+    """
+    cache, batch = _paged_call(q, k_cache, v_cache, page_table, cu_q, kv_lens, max_q)
+    n, d = q.shape[0], cache.head_dim
+    if q.dim() != 3 or q.shape[2] != d or (n and q.stride(2) != 1):
+        raise ValueError("q must be [tokens, n_q_heads, head_dim] with a contiguous last dimension")
+    if sinks is not None and (sinks.dtype != torch.float32 or sinks.shape != (q.shape[1],) or not sinks.is_contiguous()
+                              or not sinks.is_cuda):
+        raise ValueError("sinks must be fp32 [n_q_heads] on the GPU")
+    if out is None:
+        out = torch.empty(n, q.shape[1], d, dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous() or not out.is_cuda:
+        raise ValueError("out must be contiguous, like q")
+    stream = _stream(q.device)
+    ws = _paged_workspace(q.device, d, stream) if workspace is None else workspace
+    _lib.check(_lib.lib().tsb_paged_attention(
+        ctypes.byref(cache), ctypes.byref(batch), q.data_ptr(), q.stride(0), q.stride(1), q.shape[1], window,
+        keep_first, None if sinks is None else sinks.data_ptr(), d ** -0.5 if scale is None else scale,
+        out.data_ptr(), ws.data_ptr(), ws.numel(), stream))
+    return out
+
+
+def sample_tokens(logits: torch.Tensor, noise: torch.Tensor | None = None, *,
+                  temperature: torch.Tensor | None = None, top_k: torch.Tensor | None = None,
+                  top_p: torch.Tensor | None = None,
+                  min_p: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Draw one token per row of logits [B, V] (fp32 / bf16 / f16, contiguous
+    rows); returns (tokens int64 [B], logprobs fp32 [B]).
+
+    noise        fp32 [B, V] exponential variates (``torch.empty(B, V).exponential_()``): the kept token with
+                 the largest scaled logit - log(noise) is drawn.  None: every row takes its best token.
+    temperature  fp32 [B] (None: 1); rows <= 0 take their best token
+    top_k        int32 [B], <= 0: all;  top_p fp32 [B], >= 1: all;  min_p fp32 [B], <= 0: all (None: all).
+                 Equal logits rank by index; top_p counts the mass that top_k keeps; min_p is relative to
+                 the best token; the best token is always kept.
+    logprobs     of the drawn tokens under the row's softmax at its temperature, before the filters
+    """
+    _require_cuda(logits, noise, temperature, top_k, top_p, min_p)
+    if logits.dim() != 2 or logits.dtype not in _DT:
+        raise ValueError("logits must be [rows, vocabulary] of fp32, bf16 or f16")
+    rows, vocab = logits.shape
+    if vocab == 0:
+        raise ValueError("the vocabulary is empty")
+    if vocab > 1 and logits.stride(1) != 1:
+        raise ValueError("logits must have contiguous rows")
+    if noise is not None and (noise.shape != logits.shape or noise.dtype != torch.float32
+                              or (vocab > 1 and noise.stride(1) != 1)):
+        raise ValueError("noise must be fp32, shaped like logits, with contiguous rows")
+    for name, t, dt in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
+                        ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
+        if t is not None and (t.shape != (rows,) or t.dtype != dt or not t.is_contiguous()):
+            raise ValueError(f"{name} must be contiguous {dt} of one entry per row")
+    tokens = torch.empty(rows, dtype=torch.int64, device=logits.device)
+    logprobs = torch.empty(rows, dtype=torch.float32, device=logits.device)
+    row = logits.stride(0) if rows > 1 else vocab
+    noise_row = 0 if noise is None else noise.stride(0) if rows > 1 else vocab
+    _lib.check(_lib.lib().tsb_sample(
+        logits.data_ptr(), _DT[logits.dtype], rows, vocab, row, _ptr(noise), noise_row, _ptr(temperature),
+        _ptr(top_k), _ptr(top_p), _ptr(min_p), tokens.data_ptr(), logprobs.data_ptr(), _stream(logits.device)))
+    return tokens, logprobs
+
+
+# ---------------------------------------------------------------------------
 # Drop-in for torch.ops.tinyserve_ggml.ggml_mul_mat_vec
 # (tinyserve/csrc/ggml_ops.cu:461-574): same schema, argument meaning, output
 # dtype and error messages; callers ggml_forward.py:103-115 and
