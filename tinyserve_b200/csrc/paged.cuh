@@ -4,6 +4,8 @@
 #pragma once
 #include <cuda_fp8.h>
 
+#include <type_traits>
+
 #include "tsb_common.cuh"
 #include "tsb_internal.h"
 
@@ -89,8 +91,47 @@ __device__ __forceinline__ float e4m3_to_f32(uint8_t b) {
   return __half2float(*reinterpret_cast<const __half*>(&h));
 }
 
-// Workspace: the error word and counters, then the partial results of split
-// key ranges.
+// One attention call.
+struct AttnCall {
+  PagedArgs p;
+  const uint16_t* q;
+  uint16_t* out;
+  int64_t q_token_stride, q_head_stride;  // elements
+  const float* sinks;
+  unsigned* counters;  // zero between calls
+  float* part;         // partial results of split key ranges
+  float scale;
+  int window, keep_first;  // keep_first is 0 without a window
+};
+
+// A sequence with at most this many rows (new tokens x query heads of a KV
+// head) per KV head goes to the short kernel, one with more to the long one.
+constexpr int kShortRows = 16;
+
+// Workspace: the error word, the counters, the partial results.
 constexpr size_t kPagedHead = 64 * 1024;
+size_t long_partial_bytes(int head_dim);
+int launch_paged_long(const TsbPagedCache& cache, const AttnCall& c, cudaStream_t st);
+
+// Calls f with the cache's type, head size and storage as constants.
+template <class F>
+void dispatch_paged(const TsbPagedCache& c, F f) {
+  auto by_type = [&](auto dt, auto d) {
+    if (c.cache_fp8)
+      f(dt, d, std::true_type{});
+    else
+      f(dt, d, std::false_type{});
+  };
+  auto by_dim = [&](auto dt) {
+    if (c.head_dim == 64)
+      by_type(dt, std::integral_constant<int, 64>{});
+    else
+      by_type(dt, std::integral_constant<int, 128>{});
+  };
+  if (c.dtype == TSB_DT_BF16)
+    by_dim(std::integral_constant<int, TSB_DT_BF16>{});
+  else
+    by_dim(std::integral_constant<int, TSB_DT_F16>{});
+}
 
 }  // namespace tsb

@@ -8,8 +8,6 @@
 //
 //   out_t = sum_j e^(s_tj - m) v_j / (e^(sink - m) + sum_j e^(s_tj - m)),
 //   s_tj = scale * q_t . k_j,  j visible to t,  m the running maximum.
-#include <type_traits>
-
 #include "paged.cuh"
 
 namespace tsb {
@@ -126,16 +124,6 @@ __global__ void __launch_bounds__(256) paged_store_kernel(const StoreArgs s) {
 }
 
 // ------------------------------------------------------------------ attention
-struct AttnCall {
-  PagedArgs p;
-  const uint16_t* q;
-  uint16_t* out;
-  int64_t q_token_stride, q_head_stride;
-  const float* sinks;
-  float scale;
-  int window, keep_first;
-};
-
 // One warp per (token, head): the lanes split the head's dimensions, the keys
 // are walked one by one with a running maximum and sum.
 template <int DT, int D, bool FP8>
@@ -149,7 +137,7 @@ __global__ void __launch_bounds__(256) paged_attn_rows(const AttnCall c) {
   const int b = seq_of(a, token);
   if (b < 0) return;
   const SeqSpan sp = seq_span(a, b);
-  if (token - sp.q0 >= sp.q_len) return;
+  if (token - sp.q0 >= sp.q_len || sp.q_len * a.G > kShortRows) return;
   const int pos = sp.kv_len - sp.q_len + (token - sp.q0);
   const uint16_t* q = c.q + token * c.q_token_stride + head * c.q_head_stride + lane * E;
   float qv[E], o[E] = {};
@@ -245,27 +233,6 @@ int paged_args(const TsbPagedCache* c, const TsbPagedBatch* b, int n_q_heads, vo
   return TSB_OK;
 }
 
-// Calls f with the cache's type, head size and storage as constants.
-template <class F>
-void dispatch_paged(const TsbPagedCache& c, F f) {
-  auto by_type = [&](auto dt, auto d) {
-    if (c.cache_fp8)
-      f(dt, d, std::true_type{});
-    else
-      f(dt, d, std::false_type{});
-  };
-  auto by_dim = [&](auto dt) {
-    if (c.head_dim == 64)
-      by_type(dt, std::integral_constant<int, 64>{});
-    else
-      by_type(dt, std::integral_constant<int, 128>{});
-  };
-  if (c.dtype == TSB_DT_BF16)
-    by_dim(std::integral_constant<int, TSB_DT_BF16>{});
-  else
-    by_dim(std::integral_constant<int, TSB_DT_F16>{});
-}
-
 int launched() {
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? TSB_OK : fail(TSB_ERR_CUDA, cudaGetErrorString(e));
@@ -280,7 +247,7 @@ extern "C" {
 
 size_t tsb_paged_workspace(int32_t head_dim) {
   if (head_dim != 64 && head_dim != 128) return 0;
-  return kPagedHead;
+  return kPagedHead + long_partial_bytes(head_dim);
 }
 
 int tsb_paged_kv_store(const TsbPagedCache* cache, const TsbPagedBatch* batch, const void* qkv, int64_t qkv_stride,
@@ -341,8 +308,16 @@ int tsb_paged_attention(const TsbPagedCache* cache, const TsbPagedBatch* batch, 
   c.scale = scale;
   c.window = window;
   c.keep_first = window > 0 ? keep_first : 0;
-  const int64_t rows = (int64_t)batch->n_tokens * n_q_heads;
+  c.counters = static_cast<unsigned*>(workspace) + 64;
+  c.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + kPagedHead);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if ((int64_t)batch->max_q * c.p.G > kShortRows) {
+    const int rl = launch_paged_long(*cache, c, st);
+    if (rl) return rl;
+    // every sequence as long as the longest: none is short
+    if ((int64_t)batch->max_q * batch->n_seqs == batch->n_tokens) return TSB_OK;
+  }
+  const int64_t rows = (int64_t)batch->n_tokens * n_q_heads;
   dispatch_paged(*cache, [&](auto dt, auto d, auto fp8) {
     paged_attn_rows<decltype(dt)::value, decltype(d)::value, decltype(fp8)::value>
         <<<(unsigned)((rows + 7) / 8), 256, 0, st>>>(c);
