@@ -29,7 +29,7 @@
 // Warps: 0-3 and 4-7 hold the rows of the two tiles, 8 issues the products, 9
 // the tensor copies, 10-11 load Q, 12-15 load or finish K and V.  While one
 // tile's rows are in the exponential the tensor core runs the other tile's
-// products.  The rows' warps take the registers that the others give up.
+// products.
 //
 // K and V reach shared memory in one of three ways: 16-bit pools whose pages
 // hold whole groups of 8 rows by tensor copies (boxes of the largest power of
@@ -52,15 +52,12 @@ constexpr int kTileQ = 128, kTileK = 128;
 constexpr int kItemRows = 2 * kTileQ;
 constexpr int kWarpMma = 8, kWarpTma = 9, kWarpQ = 10, kQWarps = 2, kWarpKv = 12, kKvWarps = 4;
 constexpr int kThreads = 32 * (kWarpKv + kKvWarps);
-constexpr int kRowRegs = 184, kOtherRegs = 72;  // registers a thread, of 128 at launch
-static_assert(2 * kTileQ * kRowRegs + (kThreads - 2 * kTileQ) * kOtherRegs <= 128 * kThreads, "register split");
 enum Feed { kFeedTma, kFeedCopy, kFeedWiden };  // how K and V reach shared memory
 constexpr int kMaxSeqs = 512;   // sequences of one launch
 constexpr int kItemCost = 2;    // an item's fixed work in key tiles
 constexpr int kMinPiece = 6;    // a CTA's least share
 constexpr int kMaxCtas = 148;
 constexpr float kGrow = 6.f;    // rescale when the maximum grows by more (log2)
-constexpr int kPolyOf4 = 0;     // of 4 pairs of weights, those on the multiply-add units
 
 template <int D>
 constexpr int stages() {
@@ -212,14 +209,18 @@ __device__ __forceinline__ int tile_at(const Range& r, int k) { return k < r.nf 
 // Bounded; when one gives up the CTA's other waits give up too, and every
 // role falls through to the kernel's end.
 __device__ __forceinline__ bool wait_for(Shared& sh, uint64_t* bar, uint32_t parity, int32_t* err) {
+  uint32_t polls = 0;
 #pragma unroll 1
-  for (uint32_t i = 0; i < kMaxPolls; ++i) {
-    if (mbar_try_wait(bar, parity)) return true;
-    if (*reinterpret_cast<volatile int*>(&sh.abort)) return false;
+  while (!mbar_try_wait(bar, parity)) {
+    volatile int* abort = &sh.abort;
+    if (*abort) return false;
+    if (++polls == kMaxPolls) {
+      *abort = 1;
+      atomicExch(err, kDevWaitTimeout);
+      return false;
+    }
   }
-  *reinterpret_cast<volatile int*>(&sh.abort) = 1;
-  atomicExch(err, kDevWaitTimeout);
-  return false;
+  return true;
 }
 
 // The same for a whole warp, which goes on or gives up together.
@@ -257,32 +258,6 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-// 2^x of a pair on the fused multiply-add units, for x <= 100: x = n + f with
-// n the nearest integer (by adding 1.5 * 2^23) and |f| <= 1/2; 2^f by the
-// degree-4 polynomial of least largest relative error (2.6e-6, by Remez
-// exchange); times 2^n built from n's bits.  x <= -127 gives 0, NaN stays NaN.
-__device__ __forceinline__ uint64_t ex2_poly(uint64_t x) {
-  float2 v = unpair(x);
-  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(v.x));  // -127
-  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(v.y));
-  x = pair(v.x, v.y);
-  constexpr float kMagic = 12582912.f;
-  const uint64_t t = add2(x, pair(kMagic, kMagic));
-  const uint64_t f = add2(x, mul2(add2(t, pair(-kMagic, -kMagic)), pair(-1.f, -1.f)));
-  uint64_t p = pair(9.570101911e-03f, 9.570101911e-03f);
-  p = fma2(p, f, pair(5.591786032e-02f, 5.591786032e-02f));
-  p = fma2(p, f, pair(2.402474483e-01f, 2.402474483e-01f));
-  p = fma2(p, f, pair(6.931218147e-01f, 6.931218147e-01f));
-  p = fma2(p, f, pair(9.999992614e-01f, 9.999992614e-01f));
-  const float2 n = unpair(t);
-  return mul2(p, pair(__int_as_float((__float_as_int(n.x) << 23) + 0x3F800000),
-                      __int_as_float((__float_as_int(n.y) << 23) + 0x3F800000)));
 }
 template <bool F16>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
@@ -621,26 +596,13 @@ __device__ __forceinline__ bool elect_one() {
   return p != 0;
 }
 
-// f with the ring place of a K, V pair as a constant.
-template <int NP, class F>
-__device__ __forceinline__ void at_place(int place, F f) {
-  if (place == 0)
-    f(std::integral_constant<int, 0>{});
-  else if (NP == 2 || place == 1)
-    f(std::integral_constant<int, 1>{});
-  else
-    f(std::integral_constant<int, NP - 1>{});
-}
-
-// One warp walks and waits, one thread of it issues.  Its chain of waits and
-// issues is what the two tiles' rows wait for, so it is kept short: ring
-// places and Q buffers are constants of the code (addresses and descriptors
-// then cost no instructions), and each K and V is waited for once.  The order
-// of a step is QK_0(i+1), PV_1(i-1), QK_1(i+1), PV_0(i) where P lies beside S: S
-// is free for the next scores as soon as its row has been read, and the tiles
-// take turns.  Where P lies in S the step is PV_x(i), QK_x(i+1), which the
-// tensor core runs in this order.  Row warps that wait for a commit release
-// the K and V tiles and Q that it covers.
+// One warp walks and waits, one thread of it issues: its chain of waits and
+// issues is what both tiles' rows wait for, so each K and V is waited for once
+// and a product is in one place of the code.  Where P lies beside S the next
+// scores go first (S is free once its row has been read, and the row needs them
+// before it needs the sums), else PV_x(i), QK_x(i+1), which the tensor core
+// runs in this order.  Row warps that wait for a commit release the K and V
+// tiles and Q that it covers.
 template <int DT, int D, int FEED>
 __device__ void issue_products(const AttnCall& c, Shared& sh, Walk w, uint32_t q_smem, uint32_t kv_smem) {
   constexpr bool kF16 = FEED == kFeedWiden || DT == TSB_DT_F16;
@@ -648,6 +610,8 @@ __device__ void issue_products(const AttnCall& c, Shared& sh, Walk w, uint32_t q
   constexpr uint32_t kQk = idesc_f16(kTileQ, kTileK, kF16 ? 0 : 1);
   constexpr uint32_t kPv = idesc_f16(kTileQ, D, kF16 ? 0 : 1) | kIdescBTransposed;
   const bool leader = elect_one();
+  const uint64_t q_desc = sw128_desc(q_smem), k_desc = sw128_desc(kv_smem);
+  const uint64_t v_desc = sw128_mn_desc(kv_smem + TB, D == 64 ? 1024 : kTileK * 128);
   int place = 0;                // of the pair of index i, and the parity of its round
   uint32_t round = 0;
   uint32_t p_phase[2] = {0, 0}, r_phase[2] = {0, 0};
@@ -660,25 +624,18 @@ __device__ void issue_products(const AttnCall& c, Shared& sh, Walk w, uint32_t q
   const auto read_wait = [&](int x) {  // the rows have read the scores issued last
     ok = ok && warp_wait_for(sh, &sh.s_read[x], (r_phase[x] - 1) & 1, c.p.err);
   };
-  const auto qk_from = [&](auto X, auto Q, int pl) {
-    at_place<NP>(pl, [&](auto P) {
-      constexpr int x = decltype(X)::value, q = decltype(Q)::value, p = decltype(P)::value;
-#pragma unroll
-      for (int k = 0; k < D / 16; ++k) {
-        const uint32_t o = (k / 4) * (128 * 128) + (k % 4) * 32;
-        umma_f16(x * kTileK, sw128_desc(q_smem + (2 * q + x) * TB + o), sw128_desc(kv_smem + 2 * p * TB + o), kQk, k > 0);
-      }
-      umma_commit(&sh.s_full[x]);
-    });
-  };
   const auto qk = [&](auto X, int pl) {
     if (!ok) return;
     tc_fence_after();
     if (leader) {
-      if (NQ == 1 || live % 2 == 0)
-        qk_from(X, std::integral_constant<int, 0>{}, pl);
-      else
-        qk_from(X, std::integral_constant<int, NQ - 1>{}, pl);
+      constexpr int x = decltype(X)::value;
+      const uint64_t a = q_desc + (uint32_t)((live % NQ) * (2 * TB >> 4)), b = k_desc + (uint32_t)(pl * (2 * TB >> 4));
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) {
+        const uint32_t o = ((k / 4) * (128 * 128) + (k % 4) * 32) >> 4;
+        umma_f16(x * kTileK, a + x * (TB >> 4) + o, b + o, kQk, k > 0);
+      }
+      umma_commit(&sh.s_full[x]);
     }
     __syncwarp();
     ++r_phase[decltype(X)::value];
@@ -690,15 +647,11 @@ __device__ void issue_products(const AttnCall& c, Shared& sh, Walk w, uint32_t q
     ++p_phase[x];
     tc_fence_after();
     if (leader) {
-      at_place<NP>(pl, [&](auto P) {
-        constexpr int p = decltype(P)::value;
+      const uint64_t b = v_desc + (uint32_t)(pl * (2 * TB >> 4));
 #pragma unroll
-        for (int k = 0; k < kTileK / 16; ++k)
-          umma_f16_ta(o_column<D>(x), p_column<D>(x) + 8 * k,
-                      sw128_mn_desc(kv_smem + (2 * p + 1) * TB + k * 16 * 128, D == 64 ? 1024 : kTileK * 128), kPv,
-                      k > 0 || !first);
-        umma_commit(&sh.o_done[x]);
-      });
+      for (int k = 0; k < kTileK / 16; ++k)
+        umma_f16_ta(o_column<D>(x), p_column<D>(x) + 8 * k, b + (k * 16 * 128 >> 4), kPv, k > 0 || !first);
+      umma_commit(&sh.o_done[x]);
     }
     __syncwarp();
   };
@@ -710,44 +663,30 @@ __device__ void issue_products(const AttnCall& c, Shared& sh, Walk w, uint32_t q
     if (n == 0) continue;
     const bool two = s.tiles == 2;
     ok = warp_wait_for(sh, &sh.q_full[live % NQ], (live / NQ) & 1, c.p.err);
-    // step i issues the scores of index i + 1 and the sums of index i (tile 1:
-    // of i - 1 where P lies beside S); one place in the code for each product
-    int before = place;
-    const int last = p_beside_s<D>() && two ? n : n - 1;
+    // step i issues the scores of index i + 1 and the sums of index i
 #pragma unroll 1
-    for (int i = -1; i <= last && ok; ++i) {
+    for (int i = -1; i < n && ok; ++i) {
       const int next = i < 0 ? place : place + 1 == NP ? 0 : place + 1;
       const uint32_t next_round = round + (i >= 0 && next == 0);
       const bool more = i + 1 < n;
       if (more) k_wait(next, next_round);
-      if constexpr (p_beside_s<D>()) {
-        if (more) {
-          if (r_phase[0] > 0) read_wait(0);
-          qk(t0, next);
+      if (i >= 0) v_wait(place, round);
+      const auto tile = [&](auto X) {
+        if constexpr (p_beside_s<D>()) {
+          if (more) {
+            if (r_phase[decltype(X)::value] > 0) read_wait(decltype(X)::value);
+            qk(X, next);
+          }
+          if (i >= 0) pv(X, place, i == 0);
+        } else {
+          if (i >= 0) pv(X, place, i == 0);
+          if (more) qk(X, next);
         }
-        if (two && i > 0) pv(t1, before, i == 1);
-        if (two && more) {
-          if (r_phase[1] > 0) read_wait(1);
-          qk(t1, next);
-        }
-        if (i >= 0 && i < n) {
-          v_wait(place, round);
-          pv(t0, place, i == 0);
-        }
-      } else {
-        if (i >= 0) {
-          v_wait(place, round);
-          pv(t0, place, i == 0);
-        }
-        if (more) qk(t0, next);
-        if (two && i >= 0) pv(t1, place, i == 0);
-        if (two && more) qk(t1, next);
-      }
-      before = place;
-      if (i < n) {
-        place = next;
-        round = next_round;
-      }
+      };
+      tile(t0);
+      if (two) tile(t1);
+      place = next;
+      round = next_round;
     }
     ++live;
   }
@@ -888,17 +827,23 @@ __device__ void softmax_rows(const LongArgs& la, Shared& sh, Walk w, uint32_t ou
           }
           tmem_st_wait();
         }
-        uint32_t v[kTileK];
-        tmem_load_two_row64(s_at, v);
-        if constexpr (p_beside_s<D>()) {
-          tc_fence_before();
-          __syncwarp();
-          if (r % 32 == 0) mbar_arrive(&sh.s_read[x]);
-        }
+        // The row is read twice, 32 columns at a time with the next ones on their
+        // way: held whole, its 128 registers leave too few to keep the
+        // exponentials in flight.
         float mx[4] = {m, -INFINITY, -INFINITY, -INFINITY};
+        uint32_t v[2][32];
+        tmem_start_row32(s_at, v[0]);
+#pragma unroll 1
+        for (int h = 0; h < kTileK; h += 64) {
 #pragma unroll
-        for (int k = 0; k < kTileK; k += 2)
-          mx[k / 2 % 4] = max3(mx[k / 2 % 4], __uint_as_float(v[k]), __uint_as_float(v[k + 1]));
+          for (int g = 0; g < 2; ++g) {
+            tmem_finish_row32(v[g]);
+            if (g == 0 || h == 0) tmem_start_row32(s_at + h + 32 * (g + 1), v[1 - g]);
+#pragma unroll
+            for (int k = 0; k < 32; k += 2)
+              mx[k / 2 % 4] = max3(mx[k / 2 % 4], __uint_as_float(v[g][k]), __uint_as_float(v[g][k + 1]));
+          }
+        }
         const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]);
         if (__any_sync(0xffffffffu, (top - m) * cr > kGrow)) {
           const float keep = m == -INFINITY ? 0.f : ex2((m - top) * cr);
@@ -928,25 +873,31 @@ __device__ void softmax_rows(const LongArgs& la, Shared& sh, Walk w, uint32_t ou
           if (!ok) break;
           if (r == 64) release(sh, s.tiles, &sh.kv_empty[(used + 2 * i - 1) % NS]);
         }
+        tmem_start_row32(s_at, v[0]);
+#pragma unroll 1
+        for (int h = 0; h < kTileK; h += 64) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t p[32];
+          for (int g = 0; g < 2; ++g) {
+            uint32_t p[16];
+            tmem_finish_row32(v[g]);
+            if (g == 0 || h == 0) tmem_start_row32(s_at + h + 32 * (g + 1), v[1 - g]);
+            if (p_beside_s<D>() && g == 1 && h > 0) {  // the scores have been read
+              tc_fence_before();
+              __syncwarp();
+              if (r % 32 == 0) mbar_arrive(&sh.s_read[x]);
+            }
 #pragma unroll
-          for (int k = 0; k < 32; ++k) {
-            const int at = 64 * h + 2 * k;
-            const uint64_t e = fma2(pair(__uint_as_float(v[at]), __uint_as_float(v[at + 1])), cr2, mc2);
-            float2 w;
-            if (k % 4 < kPolyOf4) {
-              w = unpair(ex2_poly(e));
-            } else {
-              w = unpair(e);
+            for (int k = 0; k < 16; ++k) {
+              const uint64_t e = fma2(pair(__uint_as_float(v[g][2 * k]), __uint_as_float(v[g][2 * k + 1])), cr2, mc2);
+              float2 w = unpair(e);
               w.x = ex2(w.x);
               w.y = ex2(w.y);
+              sum[k % 2] = add2(sum[k % 2], pair(w.x, w.y));
+              p[k] = pack2<kF16>(w.x, w.y);
             }
-            sum[k % 2] = add2(sum[k % 2], pair(w.x, w.y));
-            p[k] = pack2<kF16>(w.x, w.y);
+            // where P lies in S: the columns from 32 on in S have been read
+            tmem_store_row16(p_at + h / 2 + 16 * g, p);
           }
-          tmem_store_row32(p_at + 32 * h, p);
         }
         ++o_phase;
         const float2 sums = unpair(add2(sum[0], sum[1]));
@@ -1184,10 +1135,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_long(const __grid_cons
   }
   if (works) {  // the same for the whole CTA
     if (warp < kWarpMma) {
-      asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRowRegs));
       softmax_rows<DT, D, FEED>(la, sh, w, q_smem + 2 * q_buffers<D>() * TB);
     } else {
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
       if (warp == kWarpMma) {
         issue_products<DT, D, FEED>(c, sh, w, q_smem, kv_smem);
       } else if (warp == kWarpTma) {
@@ -1265,12 +1214,7 @@ static int launch_long(LongArgs& la, const AttnCall& call, cudaStream_t st) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess && (dev >= 64 || !ready[dev])) {
-    // the registers that the row warps take must have been launched with
-    cudaFuncAttributes at;
-    e = cudaFuncGetAttributes(&at, kern);
-    if (e == cudaSuccess && at.numRegs < 128)
-      return set_error(TSB_ERR_UNSUPPORTED, "paged attention kernel built with too few registers");
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e == cudaSuccess && dev < 64) ready[dev] = true;
   }
   if (e != cudaSuccess) return set_error(TSB_ERR_CUDA, cudaGetErrorString(e));
