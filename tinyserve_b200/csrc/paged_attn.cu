@@ -1,5 +1,5 @@
-// RoPE + store into a paged KV cache, and attention of a ragged batch of new
-// tokens over it (tsb_paged_kv_store, tsb_paged_attention).
+// RoPE + store into a paged KV cache, and the entry points of the paged
+// operators (tsb_paged_kv_store, tsb_paged_attention).
 //
 // The cache is a pool of pages shared by all requests
 // (tinyserve/paged_kv_cache.py:20-122); a sliding window may keep the first
@@ -7,7 +7,11 @@
 // logit per head to the softmax denominator.
 //
 //   out_t = sum_j e^(s_tj - m) v_j / (e^(sink - m) + sum_j e^(s_tj - m)),
-//   s_tj = scale * q_t . k_j,  j visible to t,  m the running maximum.
+//   s_tj = scale * q_t . k_j,  j visible to t,  m the largest of them.
+//
+// Sequences with few rows are bound by the cache's bytes, longer chunks by
+// products and exponentials: one kernel each (paged_attn_short.cu,
+// paged_attn_long.cu); a batch with both takes two launches.
 #include "paged.cuh"
 
 namespace tsb {
@@ -123,67 +127,6 @@ __global__ void __launch_bounds__(256) paged_store_kernel(const StoreArgs s) {
   }
 }
 
-// ------------------------------------------------------------------ attention
-// One warp per (token, head): the lanes split the head's dimensions, the keys
-// are walked one by one with a running maximum and sum.
-template <int DT, int D, bool FP8>
-__global__ void __launch_bounds__(256) paged_attn_rows(const AttnCall c) {
-  const PagedArgs& a = c.p;
-  constexpr int E = D / 32;
-  const int lane = threadIdx.x & 31;
-  const int64_t w = (int64_t)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
-  if (w >= (int64_t)a.n_tokens * a.nq) return;
-  const int token = (int)(w / a.nq), head = (int)(w % a.nq);
-  const int b = seq_of(a, token);
-  if (b < 0) return;
-  const SeqSpan sp = seq_span(a, b);
-  if (token - sp.q0 >= sp.q_len || sp.q_len * a.G > kShortRows) return;
-  const int pos = sp.kv_len - sp.q_len + (token - sp.q0);
-  const uint16_t* q = c.q + token * c.q_token_stride + head * c.q_head_stride + lane * E;
-  float qv[E], o[E] = {};
-#pragma unroll
-  for (int e = 0; e < E; ++e) qv[e] = to_f32<DT>(q[e]) * c.scale;
-  float m = -INFINITY, l = 0.f;
-  const int low = c.window > 0 ? max(0, pos - c.window + 1) : 0;
-  for (int j = 0; j <= pos; ++j) {
-    if (j == min(c.keep_first, low)) j = low;  // the gap between the first tokens and the window
-    const int64_t row = cached_row(a, b, j);
-    if (row < 0) continue;
-    const int64_t at = row + (int64_t)(head / a.G) * a.head_stride + lane * E;
-    float s = 0.f, v[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      float k;
-      if constexpr (FP8) {
-        k = e4m3_to_f32(a.kc[at + e]);
-        v[e] = e4m3_to_f32(a.vc[at + e]);
-      } else {
-        k = to_f32<DT>(reinterpret_cast<const uint16_t*>(a.kc)[at + e]);
-        v[e] = to_f32<DT>(reinterpret_cast<const uint16_t*>(a.vc)[at + e]);
-      }
-      s = fmaf(qv[e], k, s);
-    }
-#pragma unroll
-    for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-    const float mn = fmaxf(m, s), base = mn == -INFINITY ? 0.f : mn;
-    const float keep = expf(m - base), p = expf(s - base);
-    l = l * keep + p;
-#pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = fmaf(p, v[e], o[e] * keep);
-    m = mn;
-  }
-  if (c.sinks) {
-    const float sink = c.sinks[head], mn = fmaxf(m, sink), base = mn == -INFINITY ? 0.f : mn, keep = expf(m - base);
-    l = l * keep + expf(sink - base);
-#pragma unroll
-    for (int e = 0; e < E; ++e) o[e] *= keep;
-  }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  uint16_t* out = c.out + ((int64_t)token * a.nq + head) * D + lane * E;
-#pragma unroll
-  for (int e = 0; e < E; ++e) out[e] = from_f32<DT>(o[e] * inv);
-}
-
 // ------------------------------------------------------------------ host
 int fail(int code, const char* what) { return set_error(code, what); }
 
@@ -239,6 +182,17 @@ int launched() {
 }
 
 }  // namespace
+
+int sm_count() {
+  static int count[64];  // by device
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 1;
+  if (dev < 64 && count[dev]) return count[dev];
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 1;
+  if (dev < 64) count[dev] = n;
+  return n;
+}
+
 }  // namespace tsb
 
 using namespace tsb;
@@ -247,7 +201,8 @@ extern "C" {
 
 size_t tsb_paged_workspace(int32_t head_dim) {
   if (head_dim != 64 && head_dim != 128) return 0;
-  return kPagedHead + long_partial_bytes(head_dim);
+  const size_t a = long_partial_bytes(head_dim), b = short_partial_bytes(head_dim);
+  return kPagedHead + (a > b ? a : b);
 }
 
 int tsb_paged_kv_store(const TsbPagedCache* cache, const TsbPagedBatch* batch, const void* qkv, int64_t qkv_stride,
@@ -317,12 +272,7 @@ int tsb_paged_attention(const TsbPagedCache* cache, const TsbPagedBatch* batch, 
     // every sequence as long as the longest: none is short
     if ((int64_t)batch->max_q * batch->n_seqs == batch->n_tokens) return TSB_OK;
   }
-  const int64_t rows = (int64_t)batch->n_tokens * n_q_heads;
-  dispatch_paged(*cache, [&](auto dt, auto d, auto fp8) {
-    paged_attn_rows<decltype(dt)::value, decltype(d)::value, decltype(fp8)::value>
-        <<<(unsigned)((rows + 7) / 8), 256, 0, st>>>(c);
-  });
-  return launched();
+  return launch_paged_short(*cache, c, st);
 }
 
 }  // extern "C"

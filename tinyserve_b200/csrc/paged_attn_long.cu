@@ -1158,16 +1158,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_long(const __grid_cons
   }
 }
 
-int sm_count() {
-  static const int n = [] {
-    int dev = 0, v = 0;
-    cudaGetDevice(&dev);
-    cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev);
-    return v;
-  }();
-  return n;
-}
-
 constexpr int part_floats(int d) { return (d + 2) * kItemRows; }
 
 }  // namespace
