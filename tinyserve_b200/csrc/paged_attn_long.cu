@@ -206,15 +206,25 @@ struct Walk {
 __device__ __forceinline__ int tile_at(const Range& r, int k) { return k < r.nf ? k : r.lo + (k - r.nf); }
 
 // ------------------------------------------------------------------ waits
-// Bounded; when one gives up the CTA's other waits give up too, and every
-// role falls through to the kernel's end.
+// Bounded (some seconds); when one gives up the CTA's other waits give up too,
+// and every role falls through to the kernel's end.
+constexpr uint32_t kPollNs = 10000, kPolls = 1u << 18;
+__device__ __forceinline__ bool phase_done(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity), "r"(kPollNs)
+      : "memory");
+  return ok != 0;
+}
 __device__ __forceinline__ bool wait_for(Shared& sh, uint64_t* bar, uint32_t parity, int32_t* err) {
   uint32_t polls = 0;
 #pragma unroll 1
-  while (!mbar_try_wait(bar, parity)) {
+  while (!phase_done(bar, parity)) {
     volatile int* abort = &sh.abort;
     if (*abort) return false;
-    if (++polls == kMaxPolls) {
+    if (++polls == kPolls) {
       *abort = 1;
       atomicExch(err, kDevWaitTimeout);
       return false;
@@ -434,13 +444,15 @@ struct Loader {
     const int64_t o = j < s.kv_len ? cached_row(c.p, s.b, j) : -1;
     return o < 0 ? -1 : o + s.head * c.p.head_stride;
   }
-  // Replaces what is not finite in this warp's rows of a V tile by zeros.
-  __device__ void clean(uint32_t base) {
+  // Replaces what is not finite in this warp's rows of a V tile by zeros; rows
+  // from `held` on hold no position (page tails, or what was there before).
+  __device__ void clean(uint32_t base, int held) {
     constexpr int CH = D / 8, RPI = 32 / CH;
     const int ch = lane % CH;
     bool any = false;
     for (int i = 0; i < kRows / RPI; ++i) {
-      const uint32_t at = base + (ch / 8) * (kTileK * 128) + sw128_off(warp * kRows + i * RPI + lane / CH, ch % 8);
+      const int row = warp * kRows + i * RPI + lane / CH;
+      const uint32_t at = base + (ch / 8) * (kTileK * 128) + sw128_off(row, ch % 8);
       uint32_t w[4];
       asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
                    : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
@@ -452,7 +464,7 @@ struct Loader {
       if (bad)
         asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
                      : "memory");
-      any |= bad;
+      any |= bad && row < held;
     }
     if (any) flag_poison();
     __syncwarp();
@@ -484,7 +496,7 @@ struct Loader {
     }
   }
   __device__ void finish_unit() {  // the copies of unit `signalled` have landed
-    if (closed_units >> (signalled % 32) & 1) clean(kv_smem + (signalled % NS) * TB);
+    if (closed_units >> (signalled % 32) & 1) clean(kv_smem + (signalled % NS) * TB, kTileK);  // zeros past the end
     announce(&sh.kv_full[signalled % NS]);
     ++signalled;
   }
@@ -578,7 +590,8 @@ struct Loader {
           const uint32_t u = unit + 1, st = u % NS;  // the V tile of this index
           ok = warp_wait_for(sh, &sh.kv_full[st], (u / NS) & 1, c.p.err);
           if (!ok) break;
-          if (!open_tile(c, p0, p1, tile_at(s.r, i) * kTileK)) clean(kv_smem + st * TB);
+          const int at = tile_at(s.r, i) * kTileK;
+          if (!open_tile(c, p0, p1, at)) clean(kv_smem + st * TB, s.kv_len - at);
           announce(&sh.v_ok[st]);
           unit += 2;
         }
@@ -693,7 +706,7 @@ __device__ void issue_products(const AttnCall& c, Shared& sh, Walk w, uint32_t q
   // nothing may be in flight when tensor memory is given back
   if (leader) {
     umma_commit(&sh.drained);
-    for (uint32_t i = 0; i < kMaxPolls && !mbar_try_wait(&sh.drained, 0); ++i) {
+    for (uint32_t i = 0; i < kPolls && !phase_done(&sh.drained, 0); ++i) {
     }
   }
   __syncwarp();
