@@ -4,10 +4,13 @@
 // Bound by the cache's bytes.  The up to 16 (token, query head) rows of a KV
 // head are one side of mma.sync m16n8k16 tiles, so each key and value is read
 // once for all of them and costs a warp no arithmetic of its own beyond its
-// share of the products.  K and V go from global memory straight to the
-// registers of the product: both products allow any order of their inner
-// dimension, and the sums any order of their columns, so a lane takes 16
-// contiguous bytes of a row and the rows of Q, and the columns of the
+// share of the products.  Each warp keeps a ring of steps (K and V of kStep
+// positions) on their way to shared memory with 16-byte asynchronous copies;
+// loaded to registers right before their use, one step at a time, the copies
+// in flight covered a third of the memory's latency (116 us for 64 tokens over
+// up to 4096 e4m3 positions).  Both products allow any order of their inner
+// dimension, and the sums any order of their columns, so a lane takes 16 (or
+// 8) contiguous bytes of a row and the rows of Q, and the columns of the
 // output, are permuted to match.
 //
 //   S = Q K^T, P = 2^(c S - c m), O = O + P V   (c = scale * log2(e))
@@ -28,7 +31,7 @@ namespace {
 
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
 constexpr int kMaxSeqs = 512;    // sequences of one launch
-constexpr int kMaxCtas = 592;    // four on each SM of a B200
+constexpr int kMaxCtas = 444;    // three on each SM of a B200
 constexpr int kItemCost = 1;     // an item's fixed work in steps
 constexpr int kMinPiece = 4;     // steps: one for each warp
 constexpr int kMaxParts = 64;    // of an item
@@ -45,10 +48,29 @@ struct ShortArgs {
   AttnCall c;
 };
 
+// A warp's ring: steps in it, bytes of a step's K or V; CTAs of an SM.
+template <int D, bool FP8>
+struct Ring {
+  static constexpr int kRowBytes = D * (FP8 ? 1 : 2);
+  static constexpr int kHalf = step_of<D>() * kRowBytes;
+  static constexpr int kSteps = FP8 ? 4 : 3;
+  static constexpr int kBytes = kWarps * kSteps * 2 * kHalf;
+  static constexpr int kPerSm = FP8 ? 3 : 2;
+};
+// Byte of 16-byte chunk c of row r: chunks of a row are exchanged so that the
+// rows and chunks that lanes read together lie in different banks.
+template <int RB>
+__device__ __forceinline__ uint32_t chunk_at(int r, int c) {
+  return RB == 64 ? r * 64 + ((c ^ (r >> 1)) & 3) * 16 : r * RB + (c ^ ((r & 6) ^ ((r & 1) << 2))) * 16;
+}
+
 template <int D>
-struct Shared {
+struct Sums {  // the four warps' results; lies over the rings
   float o[kWarps][kRows][D + 4];
   float m[kWarps][kRows], l[kWarps][kRows];
+};
+
+struct Shared {
   int q_len[kMaxSeqs], kv_len[kMaxSeqs];
   int pre[kMaxSeqs + 1];  // line length of the sequences before, per KV head
   int longest[kWarps], poison, last;
@@ -105,25 +127,19 @@ struct Segment {
   int part, parts, c_first;
 };
 
-// K and V of one step as the products take them.
 template <int DT, int D, bool FP8>
-struct Step {
-  static constexpr int STEP = step_of<D>(), NT = STEP / 8;
-  static constexpr int KW = FP8 ? D / 16 : D / 8;  // words of a lane's share of a key
-  static constexpr int VW = FP8 ? D / 32 : D / 16; // words of a lane's share of a value
-  uint32_t k[NT][KW];
-  uint32_t v[STEP / 4][VW];
-};
-
-template <int DT, int D, bool FP8>
-__global__ void __launch_bounds__(kThreads, D == 64 ? (FP8 ? 4 : 3) : 2) paged_attn_short(const __grid_constant__ ShortArgs sa) {
-  using St = Step<DT, D, FP8>;
-  constexpr int STEP = St::STEP, NT = St::NT, KW = St::KW, VW = St::VW;
+__global__ void __launch_bounds__(kThreads, Ring<D, FP8>::kPerSm) paged_attn_short(const __grid_constant__ ShortArgs sa) {
+  using Rg = Ring<D, FP8>;
+  constexpr int STEP = step_of<D>(), NT = STEP / 8, RB = Rg::kRowBytes;
+  constexpr int KW = FP8 ? D / 16 : D / 8;   // words of a lane's share of a key
+  constexpr int VW = FP8 ? D / 32 : D / 16;  // words of a lane's share of a value
   constexpr bool kF16 = FP8 || DT == TSB_DT_F16;
   constexpr float kBias = kF16 ? 8.f : 0.f;
   constexpr int EB = FP8 ? 1 : 2;
   constexpr int KS = D / 16;  // inner steps of S
-  __shared__ Shared<D> sh;
+  extern __shared__ __align__(16) uint8_t dyn[];
+  __shared__ Shared sh;
+  Sums<D>& sums = *reinterpret_cast<Sums<D>*>(dyn);
   const AttnCall& c = sa.c;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
   const int G = c.p.G;
@@ -174,7 +190,8 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? (FP8 ? 4 : 3) : 2) paged_a
     total = (int64_t)sh.pre[c.p.n_seqs] * c.p.nkv;
     if (pass == 0) {
       const int64_t share = (total + gridDim.x - 1) / gridDim.x;
-      whole = longest <= 2 * share || longest <= kMinPiece + kItemCost;
+      const int64_t items = total / max(1, longest);  // at least so many
+      whole = longest <= kMinPiece + kItemCost || (items <= gridDim.x && 8 * (int64_t)longest <= 9 * share);
       const int64_t piece = max((int64_t)kMinPiece, (int64_t)(longest + kMaxParts - 1) / kMaxParts);
       n = (int)min((int64_t)gridDim.x, max((int64_t)1, total / piece));
     } else {
@@ -280,53 +297,66 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? (FP8 ? 4 : 3) : 2) paged_a
     }
     // ---- this warp's steps
     float o[D / 8][4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-#pragma unroll 1
-    for (int k = s.k0 + warp; k < s.k1; k += kWarps) {
-      const int j0 = k < s.v.nf ? k * STEP : s.v.first + (k - s.v.nf) * STEP;
-      const int je = k < s.v.nf ? s.v.nfirst : s.kv_len;  // end of the positions of this run
+    const uint32_t ring = smem_u32(dyn) + warp * (Rg::kSteps * 2 * Rg::kHalf);
+    const auto first_of = [&](int k) { return k < s.v.nf ? k * STEP : s.v.first + (k - s.v.nf) * STEP; };
+    const auto end_of = [&](int k) { return k < s.v.nf ? s.v.nfirst : s.kv_len; };
+    const auto find = [&](int k) {  // byte offset of this lane's position of step k
       int64_t off = -1;
-      if (lane < STEP && j0 + lane < je) {
-        off = cached_row(c.p, s.b, j0 + lane);
+      if (k < s.k1 && lane < STEP && first_of(k) + lane < end_of(k)) {
+        off = cached_row(c.p, s.b, first_of(k) + lane);
         if (off >= 0) off = (off + s.head * c.p.head_stride) * EB;
       }
-      St st;
+      return off;
+    };
+    const auto fetch = [&](int k, int place, int64_t off) {
+      if (k < s.k1) {
+        constexpr int CH = RB / 16, RPI = 32 / CH;  // chunks of a row, rows a copy instruction
+        const uint32_t at = ring + place * 2 * Rg::kHalf;
 #pragma unroll
-      for (int i = 0; i < NT; ++i) {  // key 8 i + g, dims by chunks of 16 bytes: t, t + 4, ...
-        const int64_t a = __shfl_sync(0xffffffffu, off, 8 * i + g);
-#pragma unroll
-        for (int w = 0; w < KW; w += 4) {
-          uint4 r = make_uint4(0, 0, 0, 0);
-          if (a >= 0) r = __ldg(reinterpret_cast<const uint4*>(c.p.kc + a + (t + w) * 16));
-          st.k[i][w] = r.x, st.k[i][w + 1] = r.y, st.k[i][w + 2] = r.z, st.k[i][w + 3] = r.w;
+        for (int i = 0; i < STEP / RPI; ++i) {
+          const int row_i = i * RPI + lane / CH, ch = lane % CH;
+          const int64_t a = __shfl_sync(0xffffffffu, off, row_i);
+          const int64_t from = a < 0 ? 0 : a + ch * 16;
+          const uint32_t to = at + chunk_at<RB>(row_i, ch);
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(c.p.kc + from), "r"(a < 0 ? 0 : 16)
+                       : "memory");
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + Rg::kHalf), "l"(c.p.vc + from),
+                       "r"(a < 0 ? 0 : 16)
+                       : "memory");
         }
       }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
 #pragma unroll
-      for (int i = 0; i < STEP / 4; ++i) {  // value 16 (i / 4) + 2 t + {0, 1, 8, 9}, chunk g
-        const int64_t a = __shfl_sync(0xffffffffu, off, 16 * (i / 4) + 2 * t + (i & 1) + 4 * (i & 2));
-        if constexpr (VW == 2) {
-          uint2 r = make_uint2(0, 0);
-          if (a >= 0) r = __ldg(reinterpret_cast<const uint2*>(c.p.vc + a + g * 8));
-          st.v[i][0] = r.x, st.v[i][1] = r.y;
-        } else {
-#pragma unroll
-          for (int w = 0; w < VW; w += 4) {
-            uint4 r = make_uint4(0, 0, 0, 0);
-            if (a >= 0) r = __ldg(reinterpret_cast<const uint4*>(c.p.vc + a + (g + 2 * w) * 16));
-            st.v[i][w] = r.x, st.v[i][w + 1] = r.y, st.v[i][w + 2] = r.z, st.v[i][w + 3] = r.w;
-          }
-        }
-      }
+    for (int i = 0; i < Rg::kSteps - 1; ++i) fetch(s.k0 + warp + i * kWarps, i, find(s.k0 + warp + i * kWarps));
+    int64_t ahead = find(s.k0 + warp + (Rg::kSteps - 1) * kWarps);
+    int place = 0;
+#pragma unroll 1
+    for (int k = s.k0 + warp; k < s.k1; k += kWarps) {
+      const int j0 = first_of(k), je = end_of(k);
+      asm volatile("cp.async.wait_group %0;" ::"n"(Rg::kSteps - 2) : "memory");
+      __syncwarp();  // everyone's copies of this step; and the step before has been read
+      fetch(k + (Rg::kSteps - 1) * kWarps, place == 0 ? Rg::kSteps - 1 : place - 1, ahead);
+      ahead = find(k + Rg::kSteps * kWarps);
+      const uint32_t here = ring + place * 2 * Rg::kHalf;
+      place = place + 1 == Rg::kSteps ? 0 : place + 1;
       // S = Q K^T: row g (and g + 8) against keys 8 i + 2 t, + 1
       float sc[NT][4];
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
+        uint32_t kf[KW];  // key 8 i + g, dims by chunks of 16 bytes: t, t + 4, ...
+#pragma unroll
+        for (int w = 0; w < KW; w += 4)
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(kf[w]), "=r"(kf[w + 1]), "=r"(kf[w + 2]), "=r"(kf[w + 3])
+                       : "r"(here + chunk_at<RB>(8 * i + g, t + w)));
         sc[i][0] = sc[i][1] = sc[i][2] = sc[i][3] = 0.f;
 #pragma unroll
         for (int kk = 0; kk < KS; ++kk) {
           if constexpr (FP8)
-            mma<kF16>(sc[i], q[kk], e4m3x2_to_f16x2(st.k[i][kk]), e4m3x2_to_f16x2(st.k[i][kk] >> 16));
+            mma<kF16>(sc[i], q[kk], e4m3x2_to_f16x2(kf[kk]), e4m3x2_to_f16x2(kf[kk] >> 16));
           else
-            mma<kF16>(sc[i], q[kk], st.k[i][2 * kk], st.k[i][2 * kk + 1]);
+            mma<kF16>(sc[i], q[kk], kf[2 * kk], kf[2 * kk + 1]);
         }
       }
       const bool open = j0 + STEP - 1 <= base && j0 + STEP <= je &&
@@ -339,24 +369,6 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? (FP8 ? 4 : 3) : 2) paged_a
             const int j = j0 + 8 * i + 2 * t + (e & 1), p = pos[e / 2];
             if (!(j < je && j <= p && (c.window == 0 || j > p - c.window || j < c.keep_first))) sc[i][e] = -INFINITY;
           }
-        if (several) {  // a value that one row sees and another does not has to be finite
-          bool any = false;
-#pragma unroll
-          for (int i = 0; i < STEP / 4; ++i)
-#pragma unroll
-            for (int w = 0; w < VW; ++w) {
-              uint32_t bad;
-              if constexpr (FP8) {
-                bad = __vcmpeq4(st.v[i][w] & 0x7F7F7F7Fu, 0x7F7F7F7Fu);
-              } else {
-                constexpr uint32_t ex = DT == TSB_DT_F16 ? 0x7C007C00u : 0x7F807F80u;
-                bad = __vcmpeq2(st.v[i][w] & ex, ex);
-              }
-              st.v[i][w] &= ~bad;
-              any |= bad != 0;
-            }
-          if (any) sh.poison = 1;
-        }
       }
       float top[2] = {m[0], m[1]};
 #pragma unroll
@@ -397,10 +409,44 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? (FP8 ? 4 : 3) : 2) paged_a
 #pragma unroll
       for (int kk = 0; kk < STEP / 16; ++kk) {
         const uint32_t a[4] = {p[2 * kk][0], p[2 * kk][1], p[2 * kk + 1][0], p[2 * kk + 1][1]};
-        const auto& v0 = st.v[4 * kk];
-        const auto& v1 = st.v[4 * kk + 1];
-        const auto& v2 = st.v[4 * kk + 2];
-        const auto& v3 = st.v[4 * kk + 3];
+        uint32_t vf[4][VW];  // values 16 kk + 2 t + {0, 1, 8, 9}, chunk g (and g + 8)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int rv = 16 * kk + 2 * t + (i & 1) + 4 * (i & 2);
+          if constexpr (VW == 2) {
+            asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];"
+                         : "=r"(vf[i][0]), "=r"(vf[i][1])
+                         : "r"(here + Rg::kHalf + chunk_at<RB>(rv, g / 2) + (g & 1) * 8));
+          } else {
+#pragma unroll
+            for (int w = 0; w < VW; w += 4)
+              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                           : "=r"(vf[i][w]), "=r"(vf[i][w + 1]), "=r"(vf[i][w + 2]), "=r"(vf[i][w + 3])
+                           : "r"(here + Rg::kHalf + chunk_at<RB>(rv, g + 2 * w)));
+          }
+        }
+        if (!open && several) {  // a value that one row sees and another does not has to be finite
+          bool any = false;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int w = 0; w < VW; ++w) {
+              uint32_t bad;
+              if constexpr (FP8) {
+                bad = __vcmpeq4(vf[i][w] & 0x7F7F7F7Fu, 0x7F7F7F7Fu);
+              } else {
+                constexpr uint32_t ex = DT == TSB_DT_F16 ? 0x7C007C00u : 0x7F807F80u;
+                bad = __vcmpeq2(vf[i][w] & ex, ex);
+              }
+              vf[i][w] &= ~bad;
+              any |= bad != 0;
+            }
+          if (any) sh.poison = 1;
+        }
+        const auto& v0 = vf[0];
+        const auto& v1 = vf[1];
+        const auto& v2 = vf[2];
+        const auto& v3 = vf[3];
 #pragma unroll
         for (int w = 0; w < VW; ++w) {
           if constexpr (FP8) {
@@ -418,14 +464,16 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? (FP8 ? 4 : 3) : 2) paged_a
         }
       }
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();  // the rings are read: the sums take their place
     // ---- the four warps joined
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
       l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
       if (t == 0) {
-        sh.m[warp][row[h]] = m[h] == -INFINITY ? -INFINITY : m[h] * cr[h] - kBias;  // weights are 2^(c s - this)
-        sh.l[warp][row[h]] = l[h];
+        sums.m[warp][row[h]] = m[h] == -INFINITY ? -INFINITY : m[h] * cr[h] - kBias;  // weights are 2^(c s - this)
+        sums.l[warp][row[h]] = l[h];
       }
     }
 #pragma unroll
@@ -434,7 +482,7 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? (FP8 ? 4 : 3) : 2) paged_a
       for (int e = 0; e < 4; ++e) {
         const int nn = 2 * t + (e & 1);
         const int d = D == 64 ? 8 * nn + j : FP8 ? 16 * nn + j : 64 * (j / 8) + 8 * nn + j % 8;
-        sh.o[warp][row[e / 2]][d] = o[j][e];
+        sums.o[warp][row[e / 2]][d] = o[j][e];
       }
     __syncthreads();
     // thread: a row, and D / 8 of its dims
@@ -443,15 +491,15 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? (FP8 ? 4 : 3) : 2) paged_a
     const float sink = c.sinks && r < R ? c.sinks[qh] * 1.4426950408889634f : -INFINITY;
     float acc[D / 8] = {}, top = -INFINITY, sum = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sh.m[w][r]);
+    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sums.m[w][r]);
     {
       const float ref = top == -INFINITY ? 0.f : top;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        const float f = ex2(sh.m[w][r] - ref);
-        sum += sh.l[w][r] * f;
+        const float f = ex2(sums.m[w][r] - ref);
+        sum += sums.l[w][r] * f;
 #pragma unroll
-        for (int d = 0; d < D / 8; ++d) acc[d] = fmaf(f, sh.o[w][r][d0 + d], acc[d]);
+        for (int d = 0; d < D / 8; ++d) acc[d] = fmaf(f, sums.o[w][r][d0 + d], acc[d]);
       }
     }
     const bool poisoned = sh.poison != 0;
@@ -574,17 +622,27 @@ int launch_paged_short(const TsbPagedCache& cache, const AttnCall& call, cudaStr
       // no more CTAs than pieces of the least size in the longest tables
       const int64_t most = (int64_t)a.c.p.n_seqs * call.p.nkv *
                            ((call.p.max_pos / step_of<D>() + 3 + kItemCost) / kMinPiece + 1);
-      const int per_sm = D == 64 ? (FP8 ? 4 : 3) : 2;
+      auto kern = paged_attn_short<DT, D, FP8>;
+      using Rg = Ring<D, FP8>;
+      constexpr int smem = Rg::kBytes > (int)sizeof(Sums<D>) ? Rg::kBytes : (int)sizeof(Sums<D>);
+      static bool ready[64];  // by device
+      int dev = 0;
+      e = cudaGetDevice(&dev);
+      if (e == cudaSuccess && (dev >= 64 || !ready[dev]))
+        e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+      if (e != cudaSuccess) return;
+      if (dev < 64) ready[dev] = true;
       cudaLaunchConfig_t cfg = {};
-      cfg.gridDim = dim3((unsigned)min(most, (int64_t)min(kMaxCtas, per_sm * sm_count())));
+      cfg.gridDim = dim3((unsigned)min(most, (int64_t)min(kMaxCtas, Rg::kPerSm * sm_count())));
       cfg.blockDim = dim3(kThreads);
+      cfg.dynamicSmemBytes = smem;
       cfg.stream = st;
       cudaLaunchAttribute at[1];
       at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
       at[0].val.programmaticStreamSerializationAllowed = 1;
       cfg.attrs = at;
       cfg.numAttrs = 1;
-      e = cudaLaunchKernelEx(&cfg, paged_attn_short<DT, D, FP8>, a);
+      e = cudaLaunchKernelEx(&cfg, kern, a);
     }
   });
   return e == cudaSuccess ? TSB_OK : set_error(TSB_ERR_CUDA, cudaGetErrorString(e));
