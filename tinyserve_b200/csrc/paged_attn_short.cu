@@ -33,7 +33,7 @@ constexpr int kWarps = 4, kThreads = 32 * kWarps;
 constexpr int kMaxSeqs = 512;    // sequences of one launch
 constexpr int kMaxCtas = 444;    // three on each SM of a B200
 constexpr int kItemCost = 1;     // an item's fixed work in steps
-constexpr int kMinPiece = 4;     // steps: one for each warp
+constexpr int kMinPiece = 16;    // steps: four a warp; joining parts costs as much as five or six
 constexpr int kMaxParts = 64;    // of an item
 constexpr float kGrow = 6.f;
 constexpr int kRows = kShortRows;
@@ -167,6 +167,7 @@ __global__ void __launch_bounds__(kThreads, Ring<D, FP8>::kPerSm) paged_attn_sho
   int64_t total = 0;
   int n = 1;
   bool whole = false;
+#pragma unroll 1
   for (int pass = 0; pass < 2; ++pass) {
     // running sums: of steps, and again of items where a CTA takes whole ones
     if (pass == 1 && !whole) break;
@@ -200,9 +201,13 @@ __global__ void __launch_bounds__(kThreads, Ring<D, FP8>::kPerSm) paged_attn_sho
     __syncthreads();
   }
   if ((int)blockIdx.x >= n) return;
-  const auto cut = [&](int i) { return total * i / n; };
+  const bool small = total <= INT32_MAX / kMaxCtas;  // 32-bit quotients do
+  const auto ratio = [&](int64_t a, int64_t b, int64_t q) {
+    return small ? (int64_t)((uint32_t)a * (uint32_t)b / (uint32_t)q) : a * b / q;
+  };
+  const auto cut = [&](int i) { return ratio(total, i, n); };
   const auto cta_of = [&](int64_t p) {
-    int i = (int)(p * n / total);
+    int i = (int)ratio(p, n, total);
     while (i > 0 && cut(i) > p) --i;
     while (i + 1 < n && cut(i + 1) <= p) ++i;
     return i;
@@ -226,7 +231,7 @@ __global__ void __launch_bounds__(kThreads, Ring<D, FP8>::kPerSm) paged_attn_sho
       const int u = sh.pre[lo + 1] - sh.pre[lo];
       const int64_t first = (int64_t)sh.pre[lo] * c.p.nkv;
       s.b = lo;
-      s.head = (int)((x - first) / u);
+      s.head = small ? (int)((uint32_t)(x - first) / (uint32_t)u) : (int)((x - first) / u);
       s.q_len = sh.q_len[lo];
       s.kv_len = sh.kv_len[lo];
       s.v = visible<STEP>(c, s.q_len, s.kv_len);
@@ -327,9 +332,15 @@ __global__ void __launch_bounds__(kThreads, Ring<D, FP8>::kPerSm) paged_attn_sho
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
+    int64_t ahead;
+    {
+      int64_t off[Rg::kSteps];  // looked up together
 #pragma unroll
-    for (int i = 0; i < Rg::kSteps - 1; ++i) fetch(s.k0 + warp + i * kWarps, i, find(s.k0 + warp + i * kWarps));
-    int64_t ahead = find(s.k0 + warp + (Rg::kSteps - 1) * kWarps);
+      for (int i = 0; i < Rg::kSteps; ++i) off[i] = find(s.k0 + warp + i * kWarps);
+#pragma unroll
+      for (int i = 0; i < Rg::kSteps - 1; ++i) fetch(s.k0 + warp + i * kWarps, i, off[i]);
+      ahead = off[Rg::kSteps - 1];
+    }
     int place = 0;
 #pragma unroll 1
     for (int k = s.k0 + warp; k < s.k1; k += kWarps) {

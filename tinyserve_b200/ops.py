@@ -90,6 +90,14 @@ def _paged_workspace(device: torch.device, head_dim: int, stream: int) -> torch.
     return ws
 
 
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
+
+
+def _stream_of(t: torch.Tensor) -> int:
+    """The current stream of a tensor's device, without the Stream object."""
+    return _raw_stream(t.get_device()) if _raw_stream else _stream(t.device)
+
+
 def paged_device_error(workspace: torch.Tensor | None = None, device: torch.device | None = None) -> int:
     """Read and clear the device error word of a workspace, or of every
     workspace the paged operators keep for ``device``: 0 when the batches were
@@ -116,30 +124,26 @@ def _paged_call(rows: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     if not (rows.is_cuda and k_cache.is_cuda and v_cache.is_cuda and page_table.is_cuda and cu_q.is_cuda
             and kv_lens.is_cuda):
         raise RuntimeError("tinyserve_b200 kernels need CUDA tensors")
-    dtype = rows.dtype
-    if dtype not in (torch.bfloat16, torch.float16):
+    dtype, held = rows.dtype, k_cache.dtype
+    if dtype != torch.bfloat16 and dtype != torch.float16:
         raise TypeError("tokens must be bfloat16 or float16")
-    if k_cache.dtype not in (dtype, torch.float8_e4m3fn):
+    if held != dtype and held != torch.float8_e4m3fn:
         raise TypeError("the cache must hold the tokens' dtype or float8_e4m3fn")
-    ks = k_cache.stride()
-    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or ks != v_cache.stride() or v_cache.dtype != k_cache.dtype:
+    shape, strides, table = k_cache.shape, k_cache.stride(), page_table.shape
+    if len(shape) != 4 or v_cache.shape != shape or v_cache.stride() != strides or v_cache.dtype != held:
         raise ValueError("k_cache and v_cache must be alike: [pages, kv_heads, page_size, head_dim]")
-    if ks[3] != 1:
+    if strides[3] != 1:
         raise ValueError("the caches' last dimension must be contiguous")
-    n_seqs = page_table.shape[0]
-    if page_table.dim() != 2 or page_table.dtype != torch.int32 or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+    if len(table) != 2 or page_table.dtype != torch.int32 or (table[1] > 1 and page_table.stride(1) != 1):
         raise ValueError("page_table must be int32 [sequences, pages] with contiguous rows")
-    if (cu_q.dtype != torch.int32 or kv_lens.dtype != torch.int32 or cu_q.dim() != 1 or kv_lens.dim() != 1
-            or cu_q.numel() != n_seqs + 1 or kv_lens.numel() != n_seqs or not cu_q.is_contiguous()
-            or not kv_lens.is_contiguous()):
+    n_seqs, width = table
+    if (cu_q.dtype != torch.int32 or kv_lens.dtype != torch.int32 or cu_q.shape != (n_seqs + 1,)
+            or kv_lens.shape != (n_seqs,) or not cu_q.is_contiguous() or not kv_lens.is_contiguous()):
         raise ValueError("cu_q and kv_lens must be contiguous int32 of sequences + 1 and sequences entries")
-    pages, nkv, page, d = k_cache.shape
-    width = page_table.shape[1]
-    cache = _lib.TsbPagedCache(k_cache.data_ptr(), v_cache.data_ptr(), ks[0], ks[1], ks[2], pages, page, nkv, d,
-                               _DT[dtype], 1 if k_cache.element_size() == 1 else 0)
+    cache = _lib.TsbPagedCache(k_cache.data_ptr(), v_cache.data_ptr(), strides[0], strides[1], strides[2], shape[0],
+                               shape[2], shape[1], shape[3], _DT[dtype], 0 if held == dtype else 1)
     batch = _lib.TsbPagedBatch(page_table.data_ptr(), cu_q.data_ptr(), kv_lens.data_ptr(),
-                               max(width, page_table.stride(0) if n_seqs > 1 else width), width, n_seqs,
-                               rows.shape[0], max_q)
+                               page_table.stride(0) if n_seqs > 1 else width, width, n_seqs, rows.shape[0], max_q)
     return cache, batch
 
 
@@ -170,7 +174,7 @@ def paged_kv_store(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_ca
         q_out = torch.empty(n, n_q_heads, d, dtype=qkv.dtype, device=qkv.device)
     elif q_out.shape != (n, n_q_heads, d) or q_out.dtype != qkv.dtype or not q_out.is_contiguous():
         raise ValueError("q_out must be contiguous [tokens, n_q_heads, head_dim] of qkv's dtype")
-    stream = _stream(qkv.device)
+    stream = _stream_of(qkv)
     ws = _paged_workspace(qkv.device, d, stream) if workspace is None else workspace
     _lib.check(_lib.lib().tsb_paged_kv_store(
         ctypes.byref(cache), ctypes.byref(batch), qkv.data_ptr(), max(qkv.stride(0), qkv.shape[1]), n_q_heads,
@@ -203,7 +207,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         out = torch.empty(n, q.shape[1], d, dtype=q.dtype, device=q.device)
     elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous() or not out.is_cuda:
         raise ValueError("out must be contiguous, like q")
-    stream = _stream(q.device)
+    stream = _stream_of(q)
     ws = _paged_workspace(q.device, d, stream) if workspace is None else workspace
     _lib.check(_lib.lib().tsb_paged_attention(
         ctypes.byref(cache), ctypes.byref(batch), q.data_ptr(), q.stride(0), q.stride(1), q.shape[1], window,
@@ -248,7 +252,7 @@ def sample_tokens(logits: torch.Tensor, noise: torch.Tensor | None = None, *,
     noise_row = 0 if noise is None else noise.stride(0) if rows > 1 else vocab
     _lib.check(_lib.lib().tsb_sample(
         logits.data_ptr(), _DT[logits.dtype], rows, vocab, row, _ptr(noise), noise_row, _ptr(temperature),
-        _ptr(top_k), _ptr(top_p), _ptr(min_p), tokens.data_ptr(), logprobs.data_ptr(), _stream(logits.device)))
+        _ptr(top_k), _ptr(top_p), _ptr(min_p), tokens.data_ptr(), logprobs.data_ptr(), _stream_of(logits)))
     return tokens, logprobs
 
 
