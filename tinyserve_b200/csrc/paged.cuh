@@ -113,7 +113,6 @@ constexpr size_t kPagedHead = 64 * 1024;
 size_t long_partial_bytes(int head_dim);
 size_t short_partial_bytes(int head_dim);
 int launch_paged_short(const TsbPagedCache& cache, const AttnCall& c, cudaStream_t st);
-int sm_count();  // of the current device
 int launch_paged_long(const TsbPagedCache& cache, const AttnCall& c, cudaStream_t st);
 
 // Calls f with the cache's type, head size and storage as constants.

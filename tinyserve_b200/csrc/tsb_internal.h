@@ -15,6 +15,9 @@ void weight_bytes_of(int fmt, int64_t rows, int64_t cols, int64_t& data, int64_t
 
 int max_vectors_for(int K);
 
+// SMs of the current device.
+int sm_count();
+
 int launch_matvec(int fmt, const void* w, const void* s, int64_t N, int64_t K, const void* x, int xdt, int nv,
                   int64_t xs, void* y, int ydt, int64_t ys, int32_t* err, cudaStream_t st);
 int launch_gate_up(const TsbMoeSpec& sp, const TsbExpert* ex, const int32_t* ids, const void* x, float* act,
