@@ -11,15 +11,28 @@
 //
 // A cluster of CTAs shares a row: the logits come from memory once and from L2
 // in the few passes after the first.
-//   1. the best key;
-//   2. sum of w, and (for top-k, top-p) a histogram over the distance from the
-//      maximum: tokens per bin and their mass; without those filters the race;
-//   3. the bin where the k-th token or the p-th part of the mass lies; a bin with
-//      more than kList tokens is divided again by its keys, until its tokens fit
-//      a list, where each counts the tokens and the mass before it;
+//   1. the best key, and every thread's largest logit;
+//   2. the sum of w; without top-k and top-p the race as well;
+//   3. top-k: the k-th largest of the threads' maxima bounds the k-th largest
+//      logit from below, and few tokens lie above it: these are listed in one
+//      CTA, where each counts the tokens and the mass before it (top-p of them
+//      falls out of the same counts);
+//      top-p alone: a histogram of mass over the distance from the maximum, of
+//      the tokens that can matter (those below (1 - p) / vocab of the sum
+//      together weigh less than what top-p leaves out), then a list of the bin
+//      in which the limit lies.  A bin of more than kList tokens is divided
+//      again by its keys; so is the row's histogram of counts where the list of
+//      top-k does not fit.
 //   4. the race among the keys from T on; noise is read for those alone.
 // Masses are sums of integers, w in units of 2^-31, so neither the order of the
 // atomic additions nor the number of CTAs changes a result.
+//
+// One row is bound by the chain of its passes and synchronisations, many rows
+// by instructions: a pass spends a few on a token unless it may be kept.  A
+// thread copies its 16-byte pieces ahead into shared memory with a ring of
+// asynchronous copies; held in registers they were waited for when the ring
+// moved on, and loops unrolled over several loads were bound by their own
+// first fetch (58 us for a row of 201088).
 #include <cfloat>
 
 #include "tc05.cuh"
@@ -30,6 +43,8 @@ namespace tsb {
 namespace {
 
 constexpr int kThreads = 512, kWarps = kThreads / 32;
+constexpr int kRing = 8;        // 16-byte pieces of a thread under way
+constexpr int kRingBytes = kRing * kThreads * 16;
 constexpr int kBins = 1024;     // two a thread
 constexpr int kList = 1024;     // tokens that are ranked one by one
 constexpr float kPerUnit = 32;  // bins of a unit of logit: 32 units, e^-32 of the best token's weight
@@ -120,7 +135,8 @@ __device__ __forceinline__ void sync_all() {
 }
 
 template <int DT>
-__global__ void __launch_bounds__(kThreads) sample_rows(const SampleArgs a) {
+__global__ void __launch_bounds__(kThreads, 2) sample_rows(const SampleArgs a) {
+  extern __shared__ __align__(16) uint8_t ring[];
   __shared__ Shared sh;
   const int rank = (int)cluster_rank(), V = a.vocab;
   int ctas;
@@ -139,62 +155,89 @@ __global__ void __launch_bounds__(kThreads) sample_rows(const SampleArgs a) {
   const auto key_of = [&](float v, int i) { return ((uint64_t)order_bits(v) << a.index_bits) | (index_mask - i); };
   const auto index_of = [&](uint64_t key) { return (int)(index_mask - (key & index_mask)); };
 
-  // f(index, logit) of this CTA's tokens.  Loads are 16 bytes wide on 16-byte
-  // boundaries; a row that starts off them begins a few tokens early.
+  // f(index of the first, logits) of each 16 bytes of this CTA's part.  Copies
+  // lie on 16-byte boundaries; a row that starts off them begins a few tokens
+  // early, and its ends are put together token by token, -infinity outside.
   const int skew = (int)((reinterpret_cast<uintptr_t>(x) & 15) / EB);
   const int v0 = rank * a.chunk, v1 = min(v0 + a.chunk, V + skew);  // places from the boundary on
-  const auto each = [&](auto f) {
-    const uint4* src = reinterpret_cast<const uint4*>(x - skew * EB);
-    constexpr int kAhead = 4;
-    for (int b = v0 / PER + threadIdx.x; b * PER < v1; b += kAhead * kThreads) {
-      uint4 r[kAhead];
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u) {
-        const int at = (b + u * kThreads) * PER;
-        if (at >= skew && at + PER <= v1) r[u] = __ldg(src + b + u * kThreads);
-      }
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u) {
-        const int at = (b + u * kThreads) * PER;
-        if (at >= v1) break;
-        if (at >= skew && at + PER <= v1) {
-          const uint32_t w[4] = {r[u].x, r[u].y, r[u].z, r[u].w};
-#pragma unroll
-          for (int e = 0; e < PER; ++e)
-            f(at + e - skew, to_logit<DT>(PER == 4 ? w[e] : w[e / 2] >> (16 * (e & 1))));
-        } else {  // the row's ends
-          for (int e = 0; e < PER; ++e) {
-            const int i = at + e - skew;
-            if (i < 0 || i >= V) continue;
-            uint32_t bits;
-            if constexpr (EB == 4)
-              bits = reinterpret_cast<const uint32_t*>(x)[i];
-            else
-              bits = reinterpret_cast<const uint16_t*>(x)[i];
-            f(i, to_logit<DT>(bits));
-          }
-        }
+  const uint32_t mine = smem_u32(ring) + threadIdx.x * 16;
+  const auto fetch = [&](int at, int place) {
+    const uint32_t to = mine + place * (kThreads * 16);
+    if (at >= skew && at + PER <= v1) {
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(x + (int64_t)(at - skew) * EB) : "memory");
+    } else if (at < v1) {
+#pragma unroll 1
+      for (int e = 0; e < PER; ++e) {
+        const int i = at + e - skew;
+        const bool is = i >= 0 && i < V;
+        if constexpr (EB == 4)
+          asm volatile("st.shared.b32 [%0], %1;" ::"r"(to + 4 * e), "r"(is ? reinterpret_cast<const uint32_t*>(x)[i] : 0xFF800000u)
+                       : "memory");
+        else
+          asm volatile("st.shared.b16 [%0], %1;" ::"r"(to + 2 * e),
+                       "h"(is ? reinterpret_cast<const uint16_t*>(x)[i] : (uint16_t)(DT == TSB_DT_BF16 ? 0xFF80 : 0xFC00))
+                       : "memory");
       }
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  const auto each = [&](auto f) {
+    constexpr int kTurn = kThreads * PER;
+    int at = v0 + threadIdx.x * PER, place = 0;
+#pragma unroll 1
+    for (int c = 0; c < kRing - 1; ++c) fetch(at + c * kTurn, c);
+#pragma unroll 1
+    for (; at < v1; at += kTurn) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 2) : "memory");
+      uint32_t w[4];
+      asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                   : "r"(mine + place * (kThreads * 16))
+                   : "memory");
+      fetch(at + (kRing - 1) * kTurn, place == 0 ? kRing - 1 : place - 1);
+      place = place + 1 == kRing ? 0 : place + 1;
+      float v[PER];
+#pragma unroll
+      for (int e = 0; e < PER; ++e) v[e] = to_logit<DT>(PER == 4 ? w[e] : w[e / 2] >> (16 * (e & 1)));
+      f(at - skew, v);
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  };
+  // the best of the CTAs' values, read by the lanes side by side
+  const auto of_cluster = [&](const uint64_t* mine, auto f) {
+    const int lane = threadIdx.x & 31;
+    uint64_t v = remote(mine, lane < ctas ? lane : 0);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
   };
 
   // ---- 1. the best key
+  float largest = -INFINITY;  // of this thread
   uint64_t best = 0;
-  each([&](int i, float v) { best = more(best, key_of(v, i)); });
+  {
+    int at = 0;
+    each([&](int i, const float(&v)[PER]) {
+      float m = v[0];
+#pragma unroll
+      for (int e = 1; e < PER; ++e) m = fmaxf(m, v[e]);
+      if (m > largest) {
+        largest = m;
+#pragma unroll
+        for (int e = PER - 1; e >= 0; --e)
+          if (v[e] == m) at = i + e;
+      }
+    });
+    if (largest > -INFINITY) best = key_of(largest, at);
+  }
   best = block_reduce(best, more, sh.red);
   if (threadIdx.x == 0) {
     sh.best = best;
     sh.listed = 0;
   }
   sync_all();
-  for (int c = 0; c < ctas; ++c) best = more(best, remote(&sh.best, c));
-  const int first = index_of(best);
-  float top;
-  {
-    const uint32_t o = (uint32_t)(best >> a.index_bits);
-    top = __uint_as_float(o ^ ((o >> 31) ? 0x80000000u : 0xFFFFFFFFu));
-  }
-  if (top == -INFINITY) {  // the same for the whole cluster
+  best = of_cluster(&sh.best, more);
+  if (best == 0) {  // the same for the whole cluster
     if (threadIdx.x == 0 && rank == 0) {
       a.tokens[row] = -1;
       if (a.logprobs) a.logprobs[row] = -INFINITY;
@@ -202,20 +245,48 @@ __global__ void __launch_bounds__(kThreads) sample_rows(const SampleArgs a) {
     sync_all();
     return;
   }
+  const int first = index_of(best);
+  float top;
+  {
+    const uint32_t o = (uint32_t)(best >> a.index_bits);
+    top = __uint_as_float(o ^ ((o >> 31) ? 0x80000000u : 0xFFFFFFFFu));
+  }
   // (x - max) / temperature, without 0 * infinity at either end
   const auto scaled = [&](float v) {
     if (v == top) return 0.f;
     return top == INFINITY || v == -INFINITY ? -INFINITY : fmaxf(v - top, -FLT_MAX) * inv;
   };
-  // weight in units of 2^-31
-  const auto mass_of = [&](float v) { return __float2uint_rn(expf(scaled(v)) * 2147483648.f); };
+  const auto mass_of = [&](float w) { return __float2uint_rn(w * 2147483648.f); };  // in units of 2^-31
   const auto bin_of = [&](float v) {  // distance from the maximum, monotone in the logit
     const float d = v == top ? 0.f : top - v;
     return min(kBins - 1, (int)fminf(d * kPerUnit, 2e9f));
   };
-  const auto race_key = [&](int i, float v, float d) {
-    const float r = d - logf(__ldg(noise + i));
-    return key_of(r == r ? r : -INFINITY, i);
+  // the best race among 16 bytes' tokens that run: their noise is loaded
+  // together, and a fast logarithm (error below 2e-6 of scores that differ by
+  // more) tells which are worth an exact one
+  const bool wide_noise = ((reinterpret_cast<uintptr_t>(noise) / 4 - skew) & 3) == 0;
+  float ahead = -INFINITY;
+  uint64_t win = 0;
+  const auto race = [&](int i, const float(&d)[PER], const bool(&runs)[PER]) {
+    float z[PER];
+    if (wide_noise && i >= 0 && i + PER <= V) {
+#pragma unroll
+      for (int e = 0; e < PER; e += 4) {
+        const float4 q = __ldg(reinterpret_cast<const float4*>(noise + i + e));
+        z[e] = q.x, z[e + 1] = q.y, z[e + 2] = q.z, z[e + 3] = q.w;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < PER; ++e) z[e] = runs[e] ? __ldg(noise + i + e) : 1.f;
+    }
+#pragma unroll
+    for (int e = 0; e < PER; ++e)
+      if (runs[e] && !(d[e] - __logf(z[e]) < ahead - 1e-3f)) {
+        float r = d[e] - logf(z[e]);
+        r = r == r ? r : -INFINITY;
+        ahead = fmaxf(ahead, r);
+        win = more(win, key_of(r, i + e));
+      }
   };
 
   // ---- histograms: of the whole row by distance, or of one bin by keys
@@ -226,15 +297,22 @@ __global__ void __launch_bounds__(kThreads) sample_rows(const SampleArgs a) {
     for (int i = threadIdx.x; i < kBins; i += kThreads) sh.n[i] = sh.hi[i] = sh.lo[i] = 0;
     __syncthreads();
   };
-  const auto put = [&](int bin, float v) {
+  const auto put = [&](int bin, float w) {
     atomicAdd(&sh.n[bin], 1u);
     if (by_p) {
-      const uint32_t m = mass_of(v);
+      const uint32_t m = mass_of(w);
       if (m && atomicAdd(&sh.lo[bin], m) > ~m) atomicAdd(&sh.hi[bin], 1u);
     }
   };
-  const auto in_range = [&](int i, float v) {
-    if (bin_of(v) != whole_bin) return false;
+  // the tokens that a step looks at: for top-p those that top-k keeps and that
+  // weigh enough to matter
+  uint64_t floor_key = 0;
+  float lowest = -INFINITY;
+  const auto counts = [&](int i, float v) {
+    return v > -INFINITY && (floor_key == 0 || key_of(v, i) >= floor_key) && (lowest == -INFINITY || scaled(v) >= lowest);
+  };
+  const auto in_range = [&](int i, float v) {  // of these, the ones in the bin that is divided
+    if (!counts(i, v) || bin_of(v) != whole_bin) return false;
     const uint64_t key = key_of(v, i);
     return level == 0 || (key >= key_lo && key <= key_hi);
   };
@@ -244,10 +322,12 @@ __global__ void __launch_bounds__(kThreads) sample_rows(const SampleArgs a) {
     for (int b = rank * share + threadIdx.x; b < min(kBins, (rank + 1) * share); b += kThreads) {
       uint32_t n = 0;
       uint64_t m = 0;
-      for (int c = 0; c < ctas; ++c) {
-        n += remote(&sh.n[b], c);
-        if (by_p) m += ((uint64_t)remote(&sh.hi[b], c) << 32) + remote(&sh.lo[b], c);
-      }
+#pragma unroll
+      for (int c = 0; c < kMaxCluster; ++c)
+        if (c < ctas) {
+          n += remote(&sh.n[b], c);
+          if (by_p) m += ((uint64_t)remote(&sh.hi[b], c) << 32) + remote(&sh.lo[b], c);
+        }
       sh.count[b] = n;
       sh.mass[b] = m;
     }
@@ -297,50 +377,140 @@ __global__ void __launch_bounds__(kThreads) sample_rows(const SampleArgs a) {
     __syncthreads();
   };
 
-  // ---- 2. the sum of all weights, with the histogram or the race
+  // ---- 2. the sum of all weights; without filters by rank the race
   const bool filtered = by_k || by_p;
-  double sum = 0;
-  uint64_t win = 0;
-  if (filtered) clear();
+  double sum;
   {
-    double part = 0;  // so that a row's place in memory does not show in its last bit
-    each([&](int i, float v) {
-      const float d = scaled(v), w = expf(d);
-      part += w;
-      if (filtered)
-        put(bin_of(v), v);
-      else if (!greedy && (i == first || (d != -INFINITY && w >= least)))
-        win = more(win, race_key(i, v, d));
+    // two floats, so that a row's place in memory does not show in its last bit
+    float part = 0.f, rest = 0.f;
+    each([&](int i, const float(&v)[PER]) {
+      float d[PER], w[PER];
+#pragma unroll
+      for (int e = 0; e < PER; ++e) {
+        d[e] = scaled(v[e]);
+        w[e] = __expf(d[e]);
+      }
+#pragma unroll
+      for (int e = 0; e < PER; ++e) {
+        const float s = part + w[e], b = s - part;
+        rest += (part - (s - b)) + (w[e] - b);
+        part = s;
+      }
+      if (!filtered && !greedy) {
+        bool runs[PER];
+#pragma unroll
+        for (int e = 0; e < PER; ++e) runs[e] = i + e == first || (d[e] != -INFINITY && (least <= 0.f || expf(d[e]) >= least));
+        race(i, d, runs);
+      }
     });
-    sum = block_reduce(part, [](double q, double r) { return q + r; }, reinterpret_cast<double*>(sh.red));
+    sum = block_reduce((double)part + (double)rest, [](double q, double r) { return q + r; },
+                       reinterpret_cast<double*>(sh.red));
   }
   if (threadIdx.x == 0) sh.sum = sum;
+  if (filtered) sync_all();  // every CTA has to go by the same sums below
 
   // ---- 3. the threshold: top-k, then top-p of what it keeps
   uint64_t threshold = 0;
   if (filtered) {
-    combine();
-    bool whole = true;  // the histogram is the row's
-    uint64_t kept_mass = 0;
-    if (by_p) {  // of the whole row, until top-k says less
-      uint64_t m = 0;
-      for (int b = threadIdx.x; b < kBins; b += kThreads) m += remote(&sh.mass[b], b / share);
-      kept_mass = block_reduce(m, [](uint64_t q, uint64_t r) { return q + r; }, sh.red);
+    const uint32_t counter = mapa_shared(smem_u32(&sh.listed), 0), keys = mapa_shared(smem_u32(sh.list), 0),
+                   masses = mapa_shared(smem_u32(sh.list_mass), 0);
+    const auto enlist = [&](uint64_t key, float v) {  // into the first CTA's list
+      uint32_t at;
+      asm volatile("atom.shared::cluster.add.u32 %0, [%1], 1;" : "=r"(at) : "r"(counter) : "memory");
+      if (at < kList) {
+        const uint32_t m = by_p ? mass_of(expf(scaled(v))) : 0u;
+        asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(keys + 8 * at), "l"(key) : "memory");
+        asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(masses + 4 * at), "r"(m) : "memory");
+      }
+    };
+    const auto least_of = [](uint64_t q, uint64_t r) { return q < r ? q : r; };
+    bool todo_k = by_k, todo_p = by_p;
+    double kept_mass = 0;  // of what top-k keeps, or of the row
+    clear();
+    if (by_k && k <= kList) {
+      if (largest > -INFINITY) atomicAdd(&sh.n[bin_of(largest)], 1u);
+      combine();
+      scan(true, 0, 0, 0.);
+      const int bin = sh.bin;  // none: fewer threads than k have a token
+      if (bin >= 0) {
+        each([&](int i, const float(&v)[PER]) {
+#pragma unroll
+          for (int e = 0; e < PER; ++e)
+            if (v[e] > -INFINITY && bin_of(v[e]) <= bin) enlist(key_of(v[e], i + e), v[e]);
+        });
+        sync_all();
+        const int n = (int)remote(&sh.listed, 0);
+        if (n <= kList) {
+          if (rank == 0) {
+            uint64_t key[kList / kThreads], before[kList / kThreads], kept = 0;
+            uint32_t better[kList / kThreads];
+#pragma unroll
+            for (int u = 0; u < kList / kThreads; ++u) {
+              const int i = threadIdx.x + u * kThreads;
+              key[u] = i < n ? sh.list[i] : 0;
+              better[u] = 0;
+              before[u] = 0;
+              if (i < n) {
+#pragma unroll 4
+                for (int j = 0; j < n; ++j) {
+                  const bool m = sh.list[j] > key[u];
+                  better[u] += m;
+                  before[u] += m ? sh.list_mass[j] : 0u;
+                }
+                if (better[u] == (uint32_t)k - 1) {
+                  sh.result_key = key[u];
+                  sh.result_mass = before[u] + sh.list_mass[i];
+                }
+              }
+            }
+            __syncthreads();
+            if (by_p) {
+              const double want = (double)p * (double)sh.result_mass;
+              uint64_t last = sh.result_key;
+              kept = ~0ull;
+#pragma unroll
+              for (int u = 0; u < kList / kThreads; ++u)
+                if (key[u] >= last && ((double)before[u] < want || better[u] == 0)) kept = least_of(kept, key[u]);
+              kept = block_reduce(kept, least_of, sh.red);
+              if (threadIdx.x == 0) sh.result_key = kept;
+            }
+          }
+          sync_all();
+          threshold = remote(&sh.result_key, 0);
+          todo_k = todo_p = false;
+        }
+        sync_all();
+        if (threadIdx.x == 0) sh.listed = 0;
+      }
+      clear();
     }
-    for (int step = by_k ? 0 : 1; step < (by_p ? 2 : 1); ++step) {
+    bool dirty = false;  // the histogram
+    for (int step = todo_k ? 0 : 1; step < (todo_p ? 2 : 1); ++step) {
       const bool count = step == 0;
-      const double want = count ? 0. : (double)p * (double)kept_mass;
+      if (!count && !todo_k) {  // top-p of the whole row
+        double total = remote(&sh.sum, (threadIdx.x & 31) < ctas ? threadIdx.x & 31 : 0);
+        if ((threadIdx.x & 31) >= ctas) total = 0;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+        kept_mass = total * 2147483648.;
+        if (p > 0.f) lowest = logf((float)((1. - (double)p) * total / V)) - 0.01f;
+      }
+      const double want = count ? 0. : (double)p * kept_mass;
       if (!count && !(want > 0.)) {  // nothing but the first token
         threshold = best;
         break;
       }
-      if (!whole) {
-        clear();
-        each([&](int i, float v) { put(bin_of(v), v); });
-        combine();
-      }
-      whole = true;
+      if (dirty) clear();
+      dirty = true;
       level = 0;
+      floor_key = threshold;
+      each([&](int i, const float(&v)[PER]) {
+#pragma unroll
+        for (int e = 0; e < PER; ++e) {
+          if (counts(i + e, v[e])) put(bin_of(v[e]), by_p ? expf(scaled(v[e])) : 0.f);
+        }
+      });
+      combine();
       scan(count, 0, 0, want);
       while (sh.bin >= 0 && sh.bin_count > kList) {
         // divide the bin by its keys: first the span of logits that it can hold
@@ -350,57 +520,55 @@ __global__ void __launch_bounds__(kThreads) sample_rows(const SampleArgs a) {
         if (level == 0) {
           whole_bin = bin;
           uint64_t low = ~0ull, high = 0;
-          each([&](int i, float v) {
-            if (bin_of(v) != whole_bin) return;
-            const uint64_t key = key_of(v, i);
-            low = key < low ? key : low;
-            high = more(high, key);
+          each([&](int i, const float(&v)[PER]) {
+#pragma unroll
+            for (int e = 0; e < PER; ++e) {
+              if (!in_range(i + e, v[e])) continue;
+              const uint64_t key = key_of(v[e], i + e);
+              low = least_of(low, key);
+              high = more(high, key);
+            }
           });
-          low = block_reduce(low, [](uint64_t q, uint64_t r) { return q < r ? q : r; }, sh.red);
+          low = block_reduce(low, least_of, sh.red);
           high = block_reduce(high, more, sh.red);
           if (threadIdx.x == 0) {
             sh.low = low;
             sh.race = high;
           }
           sync_all();
-          for (int c = 0; c < ctas; ++c) {
-            const uint64_t l = remote(&sh.low, c);
-            low = l < low ? l : low;
-            high = more(high, remote(&sh.race, c));
-          }
-          key_lo = low;
-          key_hi = high;
+          key_lo = of_cluster(&sh.low, least_of);
+          key_hi = of_cluster(&sh.race, more);
         } else {
           key_hi -= (uint64_t)bin << shift;
           const uint64_t span = (1ull << shift) - 1;
           key_lo = key_hi - key_lo > span ? key_hi - span : key_lo;
         }
         ++level;
-        whole = false;
         shift = max(0, 64 - __clzll((long long)(key_hi - key_lo)) - 10);
         clear();
-        each([&](int i, float v) {
-          if (in_range(i, v)) put((int)((key_hi - key_of(v, i)) >> shift), v);
+        each([&](int i, const float(&v)[PER]) {
+#pragma unroll
+          for (int e = 0; e < PER; ++e)
+            if (in_range(i + e, v[e]))
+              put((int)((key_hi - key_of(v[e], i + e)) >> shift), by_p ? expf(scaled(v[e])) : 0.f);
         });
         combine();
         scan(count, bn, bm, want);
       }
-      // list the bin's tokens in the first CTA
       const int bin = sh.bin;
+      if (bin < 0) {  // fewer tokens than k; or rounding leaves the limit past the last
+        if (count) todo_k = false;
+        continue;
+      }
       const uint32_t bn = sh.before_count;
       const uint64_t bm = sh.before_mass;
       if (level == 0) whole_bin = bin;
-      const uint32_t counter = mapa_shared(smem_u32(&sh.listed), 0), keys = mapa_shared(smem_u32(sh.list), 0),
-                     masses = mapa_shared(smem_u32(sh.list_mass), 0);
-      each([&](int i, float v) {
-        if (!in_range(i, v)) return;
-        const uint64_t key = key_of(v, i);
-        if (level > 0 && (int)((key_hi - key) >> shift) != bin) return;
-        uint32_t at;
-        asm volatile("atom.shared::cluster.add.u32 %0, [%1], 1;" : "=r"(at) : "r"(counter) : "memory");
-        if (at < kList) {
-          asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(keys + 8 * at), "l"(key) : "memory");
-          asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(masses + 4 * at), "r"(by_p ? mass_of(v) : 0u) : "memory");
+      each([&](int i, const float(&v)[PER]) {
+#pragma unroll
+        for (int e = 0; e < PER; ++e) {
+          if (!in_range(i + e, v[e])) continue;
+          const uint64_t key = key_of(v[e], i + e);
+          if (level == 0 || (int)((key_hi - key) >> shift) == bin) enlist(key, v[e]);
         }
       });
       sync_all();
@@ -411,22 +579,23 @@ __global__ void __launch_bounds__(kThreads) sample_rows(const SampleArgs a) {
           const uint64_t key = sh.list[i];
           uint32_t better = 0;
           uint64_t m = bm;
-          for (int j = 0; j < n; ++j)
-            if (sh.list[j] > key) {
-              ++better;
-              m += sh.list_mass[j];
-            }
+#pragma unroll 4
+          for (int j = 0; j < n; ++j) {
+            const bool is = sh.list[j] > key;
+            better += is;
+            m += is ? sh.list_mass[j] : 0u;
+          }
           if (count) {
             if (bn + better == (uint32_t)k - 1) {
               sh.result_key = key;
               sh.result_mass = m + sh.list_mass[i];
             }
-          } else if ((double)m < want && key < last) {
-            last = key;
+          } else if ((double)m < want) {
+            last = least_of(last, key);
           }
         }
         if (!count) {
-          last = block_reduce(last, [](uint64_t q, uint64_t r) { return q < r ? q : r; }, sh.red);
+          last = block_reduce(last, least_of, sh.red);
           if (threadIdx.x == 0) sh.result_key = last;
         }
         __syncthreads();
@@ -434,33 +603,49 @@ __global__ void __launch_bounds__(kThreads) sample_rows(const SampleArgs a) {
       }
       sync_all();
       threshold = more(threshold, remote(&sh.result_key, 0));
-      if (count) kept_mass = remote(&sh.result_mass, 0);
+      if (count) kept_mass = (double)remote(&sh.result_mass, 0);
+      sync_all();
     }
 
     // ---- 4. the race of the kept
-    each([&](int i, float v) {
-      if (i != first && key_of(v, i) < threshold) return;
-      const float d = scaled(v);
-      if (i != first && (d == -INFINITY || !(expf(d) >= least))) return;
-      win = more(win, race_key(i, v, d));
+    const uint32_t edge = (uint32_t)(threshold >> a.index_bits);
+    const float floor_x = edge == 0 ? -INFINITY : __uint_as_float(edge ^ ((edge >> 31) ? 0x80000000u : 0xFFFFFFFFu));
+    each([&](int i, const float(&v)[PER]) {
+      float m = v[0];
+#pragma unroll
+      for (int e = 1; e < PER; ++e) m = fmaxf(m, v[e]);
+      if (m < floor_x) return;
+      bool runs[PER];
+      float d[PER];
+#pragma unroll
+      for (int e = 0; e < PER; ++e) {
+        d[e] = scaled(v[e]);
+        runs[e] = v[e] >= floor_x && key_of(v[e], i + e) >= threshold &&
+                  (i + e == first || (d[e] != -INFINITY && (least <= 0.f || expf(d[e]) >= least)));
+      }
+      race(i, d, runs);
     });
   }
   if (!greedy) win = block_reduce(win, more, sh.red);
   if (threadIdx.x == 0) sh.race = win;
   sync_all();
-  if (rank == 0 && threadIdx.x == 0) {
-    for (int c = 0; c < ctas; ++c) win = more(win, remote(&sh.race, c));
-    sum = 0;
-    for (int c = 0; c < ctas; ++c) sum += remote(&sh.sum, c);
-    const int token = greedy ? first : index_of(win);
-    a.tokens[row] = token;
-    if (a.logprobs) {
-      uint32_t bits;
-      if constexpr (EB == 4)
-        bits = reinterpret_cast<const uint32_t*>(x)[token];
-      else
-        bits = reinterpret_cast<const uint16_t*>(x)[token];
-      a.logprobs[row] = scaled(to_logit<DT>(bits)) - (float)log(sum);
+  if (rank == 0 && threadIdx.x < 32) {
+    win = of_cluster(&sh.race, more);
+    sum = remote(&sh.sum, threadIdx.x < ctas ? threadIdx.x : 0);
+    if (threadIdx.x >= ctas) sum = 0;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (threadIdx.x == 0) {
+      const int token = greedy ? first : index_of(win);
+      a.tokens[row] = token;
+      if (a.logprobs) {
+        uint32_t bits;
+        if constexpr (EB == 4)
+          bits = reinterpret_cast<const uint32_t*>(x)[token];
+        else
+          bits = reinterpret_cast<const uint16_t*>(x)[token];
+        a.logprobs[row] = scaled(to_logit<DT>(bits)) - logf((float)sum);
+      }
     }
   }
   sync_all();  // no CTA leaves while its memory may be read
@@ -468,9 +653,17 @@ __global__ void __launch_bounds__(kThreads) sample_rows(const SampleArgs a) {
 
 template <int DT>
 cudaError_t launch(const SampleArgs& a, int rows, int ctas, cudaStream_t st) {
+  static bool ready[64];  // by device
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && (dev >= 64 || !ready[dev]))
+    e = cudaFuncSetAttribute(sample_rows<DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes);
+  if (e != cudaSuccess) return e;
+  if (dev < 64) ready[dev] = true;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(rows * ctas);
   cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kRingBytes;
   cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -501,10 +694,9 @@ extern "C" int tsb_sample(const void* logits, int32_t dtype, int32_t rows, int32
                tokens, logprobs, row_stride,  noise_stride, vocab, 0, 1};
   while ((1 << a.index_bits) < vocab) ++a.index_bits;
   // CTAs of a row: as many as still get 4096 tokens each, fewer once the rows
-  // alone fill the GPU (a cluster's synchronisations cost about a pass over
-  // 8192 tokens)
+  // alone fill the GPU (two CTAs on an SM)
   int ctas = 1;
-  while (ctas < kMaxCluster && vocab / (2 * ctas) >= 4096 && (int64_t)rows * ctas < 4 * sm_count()) ctas *= 2;
+  while (ctas < kMaxCluster && vocab / (2 * ctas) >= 4096 && 2 * (int64_t)rows * ctas <= 2 * sm_count()) ctas *= 2;
   a.chunk = ((vocab + 8 + ctas - 1) / ctas + 7) / 8 * 8;  // 8: a row may begin off a 16-byte boundary
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const cudaError_t e = dtype == TSB_DT_F32    ? launch<TSB_DT_F32>(a, rows, ctas, st)
