@@ -12,27 +12,29 @@
 // A cluster of CTAs shares a row: the logits come from memory once and from L2
 // in the few passes after the first.
 //   1. the best key, and every thread's largest logit;
-//   2. the sum of w; without top-k and top-p the race as well;
-//   3. top-k: the k-th largest of the threads' maxima bounds the k-th largest
-//      logit from below, and few tokens lie above it: these are listed in one
-//      CTA, where each counts the tokens and the mass before it (top-p of them
-//      falls out of the same counts);
-//      top-p alone: a histogram of mass over the distance from the maximum, of
-//      the tokens that can matter (those below (1 - p) / vocab of the sum
-//      together weigh less than what top-p leaves out), then a list of the bin
-//      in which the limit lies.  A bin of more than kList tokens is divided
-//      again by its keys; so is the row's histogram of counts where the list of
-//      top-k does not fit.
+//   2. a bound below which no token can be kept: min-p gives one, top-k the k-th
+//      largest of the threads' maxima; then the sum of w and, where a bound is
+//      known, a list of the tokens above it (each warp its own).  Top-p alone
+//      takes a histogram of mass over the distance from the maximum in this
+//      pass and has its bound and lists after it.  A row without filters runs
+//      its race here;
+//   3. T, from the lists (from the whole row where a list overflows): the
+//      histogram's bin in which the limit lies, whose tokens are ranked one by
+//      one in one CTA, each counting the tokens and the mass before it.  A bin
+//      of more than kList tokens is divided again by its keys;
 //   4. the race among the keys from T on; noise is read for those alone.
 // Masses are sums of integers, w in units of 2^-31, so neither the order of the
 // atomic additions nor the number of CTAs changes a result.
 //
 // One row is bound by the chain of its passes and synchronisations, many rows
-// by instructions: a pass spends a few on a token unless it may be kept.  A
-// thread copies its 16-byte pieces ahead into shared memory with a ring of
+// by instructions.  A pass over the row therefore spends a few instructions on
+// a token, and what is done for few tokens is done from lists: in the pass, one
+// such token in a warp holds up all 32 lanes (a third of the tokens' warps with
+// one token in a hundred; 66 us for a row of 201088 with top-p).  A thread
+// copies its 16-byte pieces ahead into shared memory with a ring of
 // asynchronous copies; held in registers they were waited for when the ring
 // moved on, and loops unrolled over several loads were bound by their own
-// first fetch (58 us for a row of 201088).
+// first fetch.
 #include <cfloat>
 
 #include "tc05.cuh"
@@ -43,7 +45,8 @@ namespace tsb {
 namespace {
 
 constexpr int kThreads = 512, kWarps = kThreads / 32;
-constexpr int kRing = 8;        // 16-byte pieces of a thread under way
+constexpr int kRing = 4;        // 16-byte pieces of a thread under way
+constexpr int kOwn = 256;       // tokens of a warp's list
 constexpr int kRingBytes = kRing * kThreads * 16;
 constexpr int kBins = 1024;     // two a thread
 constexpr int kList = 1024;     // tokens that are ranked one by one
@@ -71,9 +74,11 @@ struct Shared {
   uint64_t list[kList];                     // the first CTA's: keys of the chosen bin, and their masses
   uint32_t list_mass[kList];
   uint32_t listed;
+  uint32_t own_at[kWarps][kOwn];  // the warps' lists: index and logit
+  float own[kWarps][kOwn];
   uint64_t red[kWarps], red2[kWarps];
   // read by the other CTAs
-  uint64_t best, race, low, result_key, result_mass;
+  uint64_t best, race, low, result_key, result_mass, owned;
   double sum;
   // the bin that a scan found
   int bin;
@@ -137,7 +142,7 @@ __device__ __forceinline__ void sync_all() {
 template <int DT>
 __global__ void __launch_bounds__(kThreads, 2) sample_rows(const SampleArgs a) {
   extern __shared__ __align__(16) uint8_t ring[];
-  __shared__ Shared sh;
+  Shared& sh = *reinterpret_cast<Shared*>(ring + kRingBytes);
   const int rank = (int)cluster_rank(), V = a.vocab;
   int ctas;
   asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ctas));
@@ -181,13 +186,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows(const SampleArgs a) {
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  const auto each = [&](auto f) {
+  const auto each = [&](auto f) {  // whole warps stay in the loop: outside the row they see -infinity
     constexpr int kTurn = kThreads * PER;
     int at = v0 + threadIdx.x * PER, place = 0;
+    const int ends = v1 + (threadIdx.x & 31) * PER;  // for the warp's first lane: v1
 #pragma unroll 1
     for (int c = 0; c < kRing - 1; ++c) fetch(at + c * kTurn, c);
 #pragma unroll 1
-    for (; at < v1; at += kTurn) {
+    for (; at < ends; at += kTurn) {
       asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 2) : "memory");
       uint32_t w[4];
       asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
@@ -198,7 +204,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows(const SampleArgs a) {
       place = place + 1 == kRing ? 0 : place + 1;
       float v[PER];
 #pragma unroll
-      for (int e = 0; e < PER; ++e) v[e] = to_logit<DT>(PER == 4 ? w[e] : w[e / 2] >> (16 * (e & 1)));
+      for (int e = 0; e < PER; ++e)
+        v[e] = at < v1 ? to_logit<DT>(PER == 4 ? w[e] : w[e / 2] >> (16 * (e & 1))) : -INFINITY;
       f(at - skew, v);
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
@@ -261,14 +268,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows(const SampleArgs a) {
     const float d = v == top ? 0.f : top - v;
     return min(kBins - 1, (int)fminf(d * kPerUnit, 2e9f));
   };
-  // the best race among 16 bytes' tokens that run: their noise is loaded
-  // together, and a fast logarithm (error below 2e-6 of scores that differ by
-  // more) tells which are worth an exact one
+  // A token's race; a fast logarithm (its error is far below 1e-3) tells which
+  // are worth an exact one.
   const bool wide_noise = ((reinterpret_cast<uintptr_t>(noise) / 4 - skew) & 3) == 0;
-  float ahead = -INFINITY;
-  uint64_t win = 0;
-  const auto race = [&](int i, const float(&d)[PER], const bool(&runs)[PER]) {
-    float z[PER];
+  const auto noise_of = [&](int i, const float(&v)[PER], float(&z)[PER]) {
     if (wide_noise && i >= 0 && i + PER <= V) {
 #pragma unroll
       for (int e = 0; e < PER; e += 4) {
@@ -277,16 +280,17 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows(const SampleArgs a) {
       }
     } else {
 #pragma unroll
-      for (int e = 0; e < PER; ++e) z[e] = runs[e] ? __ldg(noise + i + e) : 1.f;
+      for (int e = 0; e < PER; ++e) z[e] = v[e] > -INFINITY ? __ldg(noise + i + e) : 1.f;
     }
-#pragma unroll
-    for (int e = 0; e < PER; ++e)
-      if (runs[e] && !(d[e] - __logf(z[e]) < ahead - 1e-3f)) {
-        float r = d[e] - logf(z[e]);
-        r = r == r ? r : -INFINITY;
-        ahead = fmaxf(ahead, r);
-        win = more(win, key_of(r, i + e));
-      }
+  };
+  float ahead = -INFINITY;
+  uint64_t win = 0;
+  const auto race = [&](int i, float d, float z) {
+    if (d - __logf(z) < ahead - 1e-3f) return;
+    float r = d - logf(z);
+    r = r == r ? r : -INFINITY;
+    ahead = fmaxf(ahead, r);
+    win = more(win, key_of(r, i));
   };
 
   // ---- histograms: of the whole row by distance, or of one bin by keys
@@ -304,18 +308,51 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows(const SampleArgs a) {
       if (m && atomicAdd(&sh.lo[bin], m) > ~m) atomicAdd(&sh.hi[bin], 1u);
     }
   };
-  // the tokens that a step looks at: for top-p those that top-k keeps and that
-  // weigh enough to matter
-  uint64_t floor_key = 0;
-  float lowest = -INFINITY;
-  const auto counts = [&](int i, float v) {
-    return v > -INFINITY && (floor_key == 0 || key_of(v, i) >= floor_key) && (lowest == -INFINITY || scaled(v) >= lowest);
-  };
+  uint64_t floor_key = 0;  // top-p looks at what top-k keeps
+  const auto counts = [&](int i, float v) { return v > -INFINITY && (floor_key == 0 || key_of(v, i) >= floor_key); };
   const auto in_range = [&](int i, float v) {  // of these, the ones in the bin that is divided
     if (!counts(i, v) || bin_of(v) != whole_bin) return false;
     const uint64_t key = key_of(v, i);
     return level == 0 || (key >= key_lo && key <= key_hi);
   };
+  // ---- the warps' lists of tokens with logits from `cut` to `cap`
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int owned = 0;  // of this warp
+  float cut = -INFINITY, cap = INFINITY;
+  bool listed = false;  // the lists hold all of them, in every CTA
+  const auto own = [&](int i, const float(&v)[PER]) {
+#pragma unroll
+    for (int e = 0; e < PER; ++e) {
+      const bool is = v[e] >= cut && v[e] <= cap;
+      const uint32_t all = __ballot_sync(0xffffffffu, is);
+      if (!all) continue;
+      const int at = owned + __popc(all & ((1u << lane) - 1));
+      if (is && at < kOwn) {
+        sh.own_at[warp][at] = i + e;
+        sh.own[warp][at] = v[e];
+      }
+      owned += __popc(all);
+    }
+  };
+  const auto agree = [&] {  // whether every list of the cluster holds its tokens
+    const uint64_t most = block_reduce((uint64_t)owned, more, sh.red);
+    if (threadIdx.x == 0) sh.owned = most;
+    sync_all();
+    listed = of_cluster(&sh.owned, more) <= kOwn;
+  };
+  const auto visit = [&](auto f) {  // f(index, logit) of the lists, or of the row
+    if (listed) {
+      for (int j = lane; j < owned; j += 32) f((int)sh.own_at[warp][j], sh.own[warp][j]);
+      __syncwarp();
+    } else {
+      each([&](int i, const float(&v)[PER]) {
+#pragma unroll
+        for (int e = 0; e < PER; ++e)
+          if (v[e] > -INFINITY) f(i + e, v[e]);
+      });
+    }
+  };
+
   const int share = (kBins + ctas - 1) / ctas;  // bins that a CTA adds up
   const auto combine = [&] {
     sync_all();
@@ -377,41 +414,66 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows(const SampleArgs a) {
     __syncthreads();
   };
 
-  // ---- 2. the sum of all weights; without filters by rank the race
+  // ---- 2. what is known of the bound before the sum
   const bool filtered = by_k || by_p;
+  const bool by_min = !greedy && least > 0.f;
+  const float slack = fabsf(top) * 2.4e-7f;  // roundings of top - distance
+  clear();
+  if (by_k && k <= kList) {
+    if (largest > -INFINITY) atomicAdd(&sh.n[bin_of(largest)], 1u);
+    combine();
+    scan(true, 0, 0, 0.);
+    // none: fewer threads than k have a token.  Half a bin more than the bin's edge, for its rounding
+    if (sh.bin >= 0 && sh.bin < kBins - 1) cut = top - (sh.bin + 1.5f) / kPerUnit - slack;
+    __syncthreads();
+    clear();
+  }
+  if (by_min && !by_p) {
+    // w >= min_p: a distance of log(min_p), a little more for its rounding
+    const float d = logf(fminf(least, 1.f)) * 1.0001f - 1e-4f;
+    cut = fmaxf(cut, top + fmaxf(d / inv, -FLT_MAX) - slack);
+  }
+  if (!(cut < top)) cut = -INFINITY;  // beyond what fp32 tells apart, or infinite
+  const bool early = cut > -INFINITY;
+  const bool mass_first = by_p && !by_k;
+  // ---- the sum of all weights; without filters the race
   double sum;
   {
     // two floats, so that a row's place in memory does not show in its last bit
     float part = 0.f, rest = 0.f;
+    // (x - max) * c is enough unless it could be 0 * infinity or infinity - infinity
+    const bool plain = top < INFINITY && inv > 1e-30f && inv < 1e30f;
+    const float c = inv * 1.4426950408889634f;
     each([&](int i, const float(&v)[PER]) {
-      float d[PER], w[PER];
+      float d[PER], z[PER];
+      if (!filtered && !by_min && !greedy) noise_of(i, v, z);
 #pragma unroll
       for (int e = 0; e < PER; ++e) {
-        d[e] = scaled(v[e]);
-        w[e] = __expf(d[e]);
-      }
-#pragma unroll
-      for (int e = 0; e < PER; ++e) {
-        const float s = part + w[e], b = s - part;
-        rest += (part - (s - b)) + (w[e] - b);
+        d[e] = plain ? (v[e] - top) * inv : scaled(v[e]);
+        float w;
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(plain ? (v[e] - top) * c : d[e] * 1.4426950408889634f));
+        const float s = part + w, b = s - part;
+        rest += (part - (s - b)) + (w - b);
         part = s;
+        if (mass_first && v[e] > -INFINITY) put(bin_of(v[e]), w);
       }
-      if (!filtered && !greedy) {
-        bool runs[PER];
+      if (early) own(i, v);
+      if (!filtered && !by_min && !greedy) {
 #pragma unroll
-        for (int e = 0; e < PER; ++e) runs[e] = i + e == first || (d[e] != -INFINITY && (least <= 0.f || expf(d[e]) >= least));
-        race(i, d, runs);
+        for (int e = 0; e < PER; ++e)
+          if (i + e == first || d[e] > -INFINITY) race(i + e, scaled(v[e]), z[e]);
       }
     });
     sum = block_reduce((double)part + (double)rest, [](double q, double r) { return q + r; },
                        reinterpret_cast<double*>(sh.red));
   }
   if (threadIdx.x == 0) sh.sum = sum;
-  if (filtered) sync_all();  // every CTA has to go by the same sums below
+  if (early) agree();
 
   // ---- 3. the threshold: top-k, then top-p of what it keeps
   uint64_t threshold = 0;
   if (filtered) {
+    sync_all();  // every CTA has to go by the same sums below
     const uint32_t counter = mapa_shared(smem_u32(&sh.listed), 0), keys = mapa_shared(smem_u32(sh.list), 0),
                    masses = mapa_shared(smem_u32(sh.list_mass), 0);
     const auto enlist = [&](uint64_t key, float v) {  // into the first CTA's list
@@ -424,94 +486,45 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows(const SampleArgs a) {
       }
     };
     const auto least_of = [](uint64_t q, uint64_t r) { return q < r ? q : r; };
-    bool todo_k = by_k, todo_p = by_p;
+    bool todo_k = by_k;
     double kept_mass = 0;  // of what top-k keeps, or of the row
-    clear();
-    if (by_k && k <= kList) {
-      if (largest > -INFINITY) atomicAdd(&sh.n[bin_of(largest)], 1u);
-      combine();
-      scan(true, 0, 0, 0.);
-      const int bin = sh.bin;  // none: fewer threads than k have a token
-      if (bin >= 0) {
-        each([&](int i, const float(&v)[PER]) {
-#pragma unroll
-          for (int e = 0; e < PER; ++e)
-            if (v[e] > -INFINITY && bin_of(v[e]) <= bin) enlist(key_of(v[e], i + e), v[e]);
-        });
-        sync_all();
-        const int n = (int)remote(&sh.listed, 0);
-        if (n <= kList) {
-          if (rank == 0) {
-            uint64_t key[kList / kThreads], before[kList / kThreads], kept = 0;
-            uint32_t better[kList / kThreads];
-#pragma unroll
-            for (int u = 0; u < kList / kThreads; ++u) {
-              const int i = threadIdx.x + u * kThreads;
-              key[u] = i < n ? sh.list[i] : 0;
-              better[u] = 0;
-              before[u] = 0;
-              if (i < n) {
-#pragma unroll 4
-                for (int j = 0; j < n; ++j) {
-                  const bool m = sh.list[j] > key[u];
-                  better[u] += m;
-                  before[u] += m ? sh.list_mass[j] : 0u;
-                }
-                if (better[u] == (uint32_t)k - 1) {
-                  sh.result_key = key[u];
-                  sh.result_mass = before[u] + sh.list_mass[i];
-                }
-              }
-            }
-            __syncthreads();
-            if (by_p) {
-              const double want = (double)p * (double)sh.result_mass;
-              uint64_t last = sh.result_key;
-              kept = ~0ull;
-#pragma unroll
-              for (int u = 0; u < kList / kThreads; ++u)
-                if (key[u] >= last && ((double)before[u] < want || better[u] == 0)) kept = least_of(kept, key[u]);
-              kept = block_reduce(kept, least_of, sh.red);
-              if (threadIdx.x == 0) sh.result_key = kept;
-            }
-          }
-          sync_all();
-          threshold = remote(&sh.result_key, 0);
-          todo_k = todo_p = false;
-        }
-        sync_all();
-        if (threadIdx.x == 0) sh.listed = 0;
-      }
-      clear();
-    }
-    bool dirty = false;  // the histogram
-    for (int step = todo_k ? 0 : 1; step < (todo_p ? 2 : 1); ++step) {
+    bool ready = mass_first, dirty = mass_first;  // the histogram: of the whole row already, used
+    for (int step = by_k ? 0 : 1; step < (by_p ? 2 : 1); ++step) {
       const bool count = step == 0;
       if (!count && !todo_k) {  // top-p of the whole row
-        double total = remote(&sh.sum, (threadIdx.x & 31) < ctas ? threadIdx.x & 31 : 0);
-        if ((threadIdx.x & 31) >= ctas) total = 0;
+        double total = remote(&sh.sum, lane < ctas ? lane : 0);
+        if (lane >= ctas) total = 0;
 #pragma unroll
         for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
         kept_mass = total * 2147483648.;
-        if (p > 0.f) lowest = logf((float)((1. - (double)p) * total / V)) - 0.01f;
       }
       const double want = count ? 0. : (double)p * kept_mass;
       if (!count && !(want > 0.)) {  // nothing but the first token
         threshold = best;
         break;
       }
-      if (dirty) clear();
-      dirty = true;
       level = 0;
       floor_key = threshold;
-      each([&](int i, const float(&v)[PER]) {
-#pragma unroll
-        for (int e = 0; e < PER; ++e) {
-          if (counts(i + e, v[e])) put(bin_of(v[e]), by_p ? expf(scaled(v[e])) : 0.f);
-        }
-      });
+      if (!ready) {
+        if (dirty) clear();
+        visit([&](int i, float v) {
+          if (counts(i, v)) put(bin_of(v), by_p ? expf(scaled(v)) : 0.f);
+        });
+      }
+      ready = false;
+      dirty = true;
       combine();
       scan(count, 0, 0, want);
+      if (!listed && sh.bin >= 0 && sh.bin < kBins - 1) {
+        // lists of what may be kept; where that is too much, of the bin alone
+        cut = top - (sh.bin + 1.5f) / kPerUnit - slack;
+        for (int only = 0; only < 2 && !listed && cut < top && cut > -INFINITY; ++only) {
+          if (only) cap = fminf(top, top - (sh.bin - 0.5f) / kPerUnit + slack);
+          owned = 0;
+          each(own);
+          agree();
+        }
+      }
       while (sh.bin >= 0 && sh.bin_count > kList) {
         // divide the bin by its keys: first the span of logits that it can hold
         const int bin = sh.bin;
@@ -520,14 +533,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows(const SampleArgs a) {
         if (level == 0) {
           whole_bin = bin;
           uint64_t low = ~0ull, high = 0;
-          each([&](int i, const float(&v)[PER]) {
-#pragma unroll
-            for (int e = 0; e < PER; ++e) {
-              if (!in_range(i + e, v[e])) continue;
-              const uint64_t key = key_of(v[e], i + e);
-              low = least_of(low, key);
-              high = more(high, key);
-            }
+          visit([&](int i, float v) {
+            if (!in_range(i, v)) return;
+            const uint64_t key = key_of(v, i);
+            low = least_of(low, key);
+            high = more(high, key);
           });
           low = block_reduce(low, least_of, sh.red);
           high = block_reduce(high, more, sh.red);
@@ -546,11 +556,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows(const SampleArgs a) {
         ++level;
         shift = max(0, 64 - __clzll((long long)(key_hi - key_lo)) - 10);
         clear();
-        each([&](int i, const float(&v)[PER]) {
-#pragma unroll
-          for (int e = 0; e < PER; ++e)
-            if (in_range(i + e, v[e]))
-              put((int)((key_hi - key_of(v[e], i + e)) >> shift), by_p ? expf(scaled(v[e])) : 0.f);
+        visit([&](int i, float v) {
+          if (in_range(i, v)) put((int)((key_hi - key_of(v, i)) >> shift), by_p ? expf(scaled(v)) : 0.f);
         });
         combine();
         scan(count, bn, bm, want);
@@ -563,13 +570,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows(const SampleArgs a) {
       const uint32_t bn = sh.before_count;
       const uint64_t bm = sh.before_mass;
       if (level == 0) whole_bin = bin;
-      each([&](int i, const float(&v)[PER]) {
-#pragma unroll
-        for (int e = 0; e < PER; ++e) {
-          if (!in_range(i + e, v[e])) continue;
-          const uint64_t key = key_of(v[e], i + e);
-          if (level == 0 || (int)((key_hi - key) >> shift) == bin) enlist(key, v[e]);
-        }
+      visit([&](int i, float v) {
+        if (!in_range(i, v)) return;
+        const uint64_t key = key_of(v, i);
+        if (level == 0 || (int)((key_hi - key) >> shift) == bin) enlist(key, v);
       });
       sync_all();
       if (rank == 0) {
@@ -603,27 +607,33 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows(const SampleArgs a) {
       }
       sync_all();
       threshold = more(threshold, remote(&sh.result_key, 0));
+      if (cap < INFINITY) listed = false;  // the lists are of no further use
+      cap = INFINITY;
       if (count) kept_mass = (double)remote(&sh.result_mass, 0);
       sync_all();
     }
 
-    // ---- 4. the race of the kept
+  }
+  // ---- 4. the race of the kept
+  if ((filtered || by_min) && listed) {
+    visit([&](int i, float v) {
+      if (i != first && key_of(v, i) < threshold) return;
+      const float d = scaled(v);
+      if (i == first || (d > -INFINITY && (least <= 0.f || expf(d) >= least))) race(i, d, __ldg(noise + i));
+    });
+  } else if (filtered || by_min) {
+    // many are kept: a pass over the row with its noise
     const uint32_t edge = (uint32_t)(threshold >> a.index_bits);
     const float floor_x = edge == 0 ? -INFINITY : __uint_as_float(edge ^ ((edge >> 31) ? 0x80000000u : 0xFFFFFFFFu));
     each([&](int i, const float(&v)[PER]) {
-      float m = v[0];
-#pragma unroll
-      for (int e = 1; e < PER; ++e) m = fmaxf(m, v[e]);
-      if (m < floor_x) return;
-      bool runs[PER];
-      float d[PER];
+      float z[PER];
+      noise_of(i, v, z);
 #pragma unroll
       for (int e = 0; e < PER; ++e) {
-        d[e] = scaled(v[e]);
-        runs[e] = v[e] >= floor_x && key_of(v[e], i + e) >= threshold &&
-                  (i + e == first || (d[e] != -INFINITY && (least <= 0.f || expf(d[e]) >= least)));
+        const float d = scaled(v[e]);
+        const bool kept = v[e] > floor_x || (v[e] == floor_x && key_of(v[e], i + e) >= threshold);
+        if (i + e == first || (kept && d > -INFINITY && (least <= 0.f || expf(d) >= least))) race(i + e, d, z[e]);
       }
-      race(i, d, runs);
     });
   }
   if (!greedy) win = block_reduce(win, more, sh.red);
@@ -657,13 +667,14 @@ cudaError_t launch(const SampleArgs& a, int rows, int ctas, cudaStream_t st) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess && (dev >= 64 || !ready[dev]))
-    e = cudaFuncSetAttribute(sample_rows<DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes);
+    e = cudaFuncSetAttribute(sample_rows<DT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             kRingBytes + (int)sizeof(Shared));
   if (e != cudaSuccess) return e;
   if (dev < 64) ready[dev] = true;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(rows * ctas);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = kRingBytes;
+  cfg.dynamicSmemBytes = kRingBytes + sizeof(Shared);
   cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -693,10 +704,11 @@ extern "C" int tsb_sample(const void* logits, int32_t dtype, int32_t rows, int32
   SampleArgs a{logits, noise,  temperature, top_k,        top_p, min_p,
                tokens, logprobs, row_stride,  noise_stride, vocab, 0, 1};
   while ((1 << a.index_bits) < vocab) ++a.index_bits;
-  // CTAs of a row: as many as still get 4096 tokens each, fewer once the rows
-  // alone fill the GPU (two CTAs on an SM)
+  // CTAs of a row: as many as still get 4096 tokens each, until the rows' CTAs
+  // reach the SMs (64 rows of 201088, mixed: 2 CTAs 215 us, 8 CTAs 180 us; 200 rows
+  // of 32001, top-k: 1 CTA 37 us, 2 CTAs 46 us)
   int ctas = 1;
-  while (ctas < kMaxCluster && vocab / (2 * ctas) >= 4096 && 2 * (int64_t)rows * ctas <= 2 * sm_count()) ctas *= 2;
+  while (ctas < kMaxCluster && vocab / (2 * ctas) >= 4096 && (int64_t)rows * ctas < sm_count()) ctas *= 2;
   a.chunk = ((vocab + 8 + ctas - 1) / ctas + 7) / 8 * 8;  // 8: a row may begin off a 16-byte boundary
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const cudaError_t e = dtype == TSB_DT_F32    ? launch<TSB_DT_F32>(a, rows, ctas, st)
