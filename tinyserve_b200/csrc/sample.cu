@@ -49,7 +49,8 @@ constexpr int kRing = 4;        // 16-byte pieces of a thread under way
 constexpr int kOwn = 256;       // tokens of a warp's list
 constexpr int kRingBytes = kRing * kThreads * 16;
 constexpr int kBins = 1024;     // two a thread
-constexpr int kList = 1024;     // tokens that are ranked one by one
+constexpr int kList = 256;      // tokens that are ranked one by one; 800 of them took longer than two more divisions
+constexpr int kMaxima = 1024;   // largest k that the threads' maxima are asked about
 constexpr float kPerUnit = 32;  // bins of a unit of logit: 32 units, e^-32 of the best token's weight
 constexpr int kMaxCluster = 8;
 
@@ -321,6 +322,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows(const SampleArgs a) {
   float cut = -INFINITY, cap = INFINITY;
   bool listed = false;  // the lists hold all of them, in every CTA
   const auto own = [&](int i, const float(&v)[PER]) {
+    if (owned > kOwn) return;  // full: it does not matter by how much
 #pragma unroll
     for (int e = 0; e < PER; ++e) {
       const bool is = v[e] >= cut && v[e] <= cap;
@@ -419,7 +421,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows(const SampleArgs a) {
   const bool by_min = !greedy && least > 0.f;
   const float slack = fabsf(top) * 2.4e-7f;  // roundings of top - distance
   clear();
-  if (by_k && k <= kList) {
+  if (by_k && k <= kMaxima) {
     if (largest > -INFINITY) atomicAdd(&sh.n[bin_of(largest)], 1u);
     combine();
     scan(true, 0, 0, 0.);
