@@ -79,7 +79,10 @@ def paged_workspace(device: torch.device, head_dim: int) -> torch.Tensor:
     """Zero-initialised scratch of the paged operators.  One workspace serves
     successive calls on one stream; the operators keep one per (device,
     stream) unless they are given another."""
-    return torch.zeros(_lib.lib().tsb_paged_workspace(head_dim), dtype=torch.uint8, device=device)
+    n = _lib.lib().tsb_paged_workspace(head_dim)
+    if n == 0:
+        raise RuntimeError("head_dim must be 64 or 128")
+    return torch.zeros(n, dtype=torch.uint8, device=device)
 
 
 def _paged_workspace(device: torch.device, head_dim: int, stream: int) -> torch.Tensor:
