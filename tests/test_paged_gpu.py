@@ -278,6 +278,28 @@ def test_store(ops, d, dtype, tables, held):
         assert torch.equal(pool.float()[keep], before.float()[keep])
 
 
+@pytest.mark.parametrize("dtype", [BF, F16])
+def test_store_beyond_the_range_of_e4m3(ops, dtype):
+    """Values around and past 448, infinities and NaN become what a plain cast makes of them."""
+    x = torch.tensor([447.0, 448.0, 456.0, 464.0, 465.0, 466.0, 480.0, 1000.0, 6e4, float("inf"), float("nan"), 0.0,
+                      2.0 ** -9, 2.0 ** -10, 1.5 * 2.0 ** -10, 2.0 ** -14, 17.3, 0.013])
+    x = torch.cat([x, -x, torch.linspace(-470, 470, 28)]).to(dtype).cuda()
+    qkv = torch.zeros(1, 3 * 64, dtype=dtype, device="cuda")
+    qkv[0, 64:128], qkv[0, 128:] = x, x.flip(0)
+    one, zero = torch.ones(1, 32, device="cuda"), torch.zeros(1, 32, device="cuda")
+    k = torch.zeros(1, 1, 16, 64, dtype=E4, device="cuda")
+    v = torch.zeros_like(k)
+    table = torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+    cu, kv = torch.tensor([0, 1], dtype=torch.int32).cuda(), torch.ones(1, dtype=torch.int32).cuda()
+    ops.paged_kv_store(qkv, one, zero, k, v, table, cu, kv, n_q_heads=1)
+    want = qkv[0].to(E4).float()
+    fin = torch.isfinite(x.float())  # x * 1 - y * 0 is NaN next to an infinity, in the other half too
+    fin = fin & fin.roll(32)
+    assert torch.equal(v[0, 0, 0].float().nan_to_num(nan=-1.0), want[128:].nan_to_num(nan=-1.0))
+    assert torch.equal(k[0, 0, 0].float()[fin].nan_to_num(nan=-1.0), want[64:128][fin].nan_to_num(nan=-1.0))
+    assert torch.isnan(k[0, 0, 0].float()[~fin]).all()
+
+
 def test_store_then_attend(ops):
     """A prompt in chunks through both operators equals it in one go."""
     nq, nkv, d, n = 8, 2, 64, 150

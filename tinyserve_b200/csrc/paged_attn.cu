@@ -18,10 +18,14 @@ namespace tsb {
 namespace {
 
 // ------------------------------------------------------------------ store
-// One CTA per token; a thread takes 8 dims of a head's lower half with the 8
-// of its upper half (two 16-byte loads, two 16-byte stores), so rotation
-// needs no exchange.  Products and sums are rounded one by one in fp32 (no
-// contraction), then once to the 16-bit type.
+// Bound by the bytes of the rows.  A thread takes 8 dims of a head's lower half
+// with the 8 of its upper half (two 16-byte loads, two 16-byte stores), so
+// rotation needs no exchange, for every 32nd (D = 64) or 16th head of its
+// token: the table's values are read once for all of them, and up to four
+// heads' loads are under way together, ahead of the look-ups of sequence and
+// page that the stores wait for.  Products and sums are rounded one by one in
+// fp32 (no contraction), then once to the 16-bit type.
+constexpr int kStoreToken = 128;  // threads of a token
 struct StoreArgs {
   PagedArgs p;
   const uint16_t* qkv;
@@ -59,15 +63,22 @@ __device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// 8 values of the 16-bit type, rounded once more to e4m3.
+// 8 values of the 16-bit type, rounded once more to e4m3.  The hardware's
+// conversion saturates; a plain cast makes NaN (with the value's sign) of what
+// rounds past 448, that is of what lies above 464.
 template <int DT>
 __device__ __forceinline__ uint2 pack8_e4m3(uint4 v) {
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
   uint32_t o[2] = {0, 0};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float f = to_f32<DT>((uint16_t)(w[i / 2] >> (16 * (i & 1))));
-    o[i / 4] |= (uint32_t)__nv_cvt_float_to_fp8(f, __NV_NOSAT, __NV_E4M3) << (8 * (i & 3));
+  for (int i = 0; i < 4; ++i) {
+    const float lo = to_f32<DT>((uint16_t)w[i]), hi = to_f32<DT>((uint16_t)(w[i] >> 16));
+    uint16_t b;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(b) : "f"(hi), "f"(lo));
+    uint32_t two = b;
+    if (!(fabsf(lo) <= 464.f)) two |= 0x007Fu;
+    if (!(fabsf(hi) <= 464.f)) two |= 0x7F00u;
+    o[i / 2] |= two << (16 * (i & 1));
   }
   return make_uint2(o[0], o[1]);
 }
@@ -76,52 +87,71 @@ template <int DT, int D, bool FP8, bool TF32>
 __global__ void __launch_bounds__(256) paged_store_kernel(const StoreArgs s) {
   const PagedArgs& a = s.p;
   constexpr int kC = D / 16;  // 8-dim chunks of a half
-  const int token = blockIdx.x;
+  constexpr int kSlots = kStoreToken / kC, kAhead = 4;
+  const int token = blockIdx.x * (256 / kStoreToken) + threadIdx.x / kStoreToken;
+  if (token >= a.n_tokens) return;
+  const int c = threadIdx.x % kC, slot = threadIdx.x % kStoreToken / kC, heads = a.nq + 2 * a.nkv;
+  const uint16_t* src = s.qkv + (int64_t)token * s.qkv_stride + c * 8;
+  uint4 r1[kAhead], r2[kAhead];
+  const auto load = [&](int first) {
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int head = first + u * kSlots;
+      if (head < heads) {
+        r1[u] = *reinterpret_cast<const uint4*>(src + head * D);
+        r2[u] = *reinterpret_cast<const uint4*>(src + head * D + D / 2);
+      }
+    }
+  };
+  load(slot);
   const int b = seq_of(a, token);
   if (b < 0) return;
   const SeqSpan sp = seq_span(a, b);
   const int pos = sp.kv_len - sp.q_len + (token - sp.q0);
   if (token - sp.q0 >= sp.q_len) return;  // a span that was reported and cut
   if (pos < 0 || pos >= s.max_rope) {
-    if (threadIdx.x == 0) atomicExch(a.err, kDevBadPlan);
+    if (threadIdx.x % kStoreToken == 0) atomicExch(a.err, kDevBadPlan);
     return;
   }
+  float cs[8], sn[8];
+  load_table8<DT, TF32>(s.cos, (int64_t)pos * (D / 2) + c * 8, cs);
+  load_table8<DT, TF32>(s.sin, (int64_t)pos * (D / 2) + c * 8, sn);
   const int64_t row = cached_row(a, b, pos);
-  const uint16_t* src = s.qkv + (int64_t)token * s.qkv_stride;
-  for (int u = threadIdx.x; u < (a.nq + 2 * a.nkv) * kC; u += blockDim.x) {
-    const int head = u / kC, c = u - head * kC;
-    const uint4 r1 = *reinterpret_cast<const uint4*>(src + head * D + c * 8);
-    const uint4 r2 = *reinterpret_cast<const uint4*>(src + head * D + D / 2 + c * 8);
-    uint4 o1 = r1, o2 = r2;
-    if (head < a.nq + a.nkv) {
-      float cs[8], sn[8], y1[8], y2[8];
-      load_table8<DT, TF32>(s.cos, (int64_t)pos * (D / 2) + c * 8, cs);
-      load_table8<DT, TF32>(s.sin, (int64_t)pos * (D / 2) + c * 8, sn);
-      const uint32_t w1[4] = {r1.x, r1.y, r1.z, r1.w}, w2[4] = {r2.x, r2.y, r2.z, r2.w};
+  for (int first = slot; first < heads; first += kAhead * kSlots) {
+    if (first > slot) load(first);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float x1 = to_f32<DT>((uint16_t)(w1[i / 2] >> (16 * (i & 1))));
-        const float x2 = to_f32<DT>((uint16_t)(w2[i / 2] >> (16 * (i & 1))));
-        y1[i] = __fsub_rn(__fmul_rn(x1, cs[i]), __fmul_rn(x2, sn[i]));
-        y2[i] = __fadd_rn(__fmul_rn(x2, cs[i]), __fmul_rn(x1, sn[i]));
+    for (int u = 0; u < kAhead; ++u) {
+      const int head = first + u * kSlots;
+      if (head >= heads) break;
+      uint4 o1 = r1[u], o2 = r2[u];
+      if (head < a.nq + a.nkv) {
+        float y1[8], y2[8];
+        const uint32_t w1[4] = {o1.x, o1.y, o1.z, o1.w}, w2[4] = {o2.x, o2.y, o2.z, o2.w};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float x1 = to_f32<DT>((uint16_t)(w1[i / 2] >> (16 * (i & 1))));
+          const float x2 = to_f32<DT>((uint16_t)(w2[i / 2] >> (16 * (i & 1))));
+          y1[i] = __fsub_rn(__fmul_rn(x1, cs[i]), __fmul_rn(x2, sn[i]));
+          y2[i] = __fadd_rn(__fmul_rn(x2, cs[i]), __fmul_rn(x1, sn[i]));
+        }
+        o1 = pack8<DT>(y1);
+        o2 = pack8<DT>(y2);
       }
-      o1 = pack8<DT>(y1);
-      o2 = pack8<DT>(y2);
-    }
-    if (head < a.nq) {
-      uint16_t* q = s.q_out + ((int64_t)token * a.nq + head) * D;
-      *reinterpret_cast<uint4*>(q + c * 8) = o1;
-      *reinterpret_cast<uint4*>(q + D / 2 + c * 8) = o2;
-    } else if (row >= 0) {
-      const bool key = head < a.nq + a.nkv;
-      const int64_t at = row + (int64_t)(head - a.nq - (key ? 0 : a.nkv)) * a.head_stride + c * 8;
-      uint8_t* pool = const_cast<uint8_t*>(key ? a.kc : a.vc);
-      if constexpr (FP8) {
-        *reinterpret_cast<uint2*>(pool + at) = pack8_e4m3<DT>(o1);
-        *reinterpret_cast<uint2*>(pool + at + D / 2) = pack8_e4m3<DT>(o2);
-      } else {
-        *reinterpret_cast<uint4*>(pool + 2 * at) = o1;
-        *reinterpret_cast<uint4*>(pool + 2 * (at + D / 2)) = o2;
+      if (head < a.nq) {
+        uint16_t* q = s.q_out + ((int64_t)token * a.nq + head) * D + c * 8;
+        *reinterpret_cast<uint4*>(q) = o1;
+        *reinterpret_cast<uint4*>(q + D / 2) = o2;
+      } else if (row >= 0) {
+        const bool key = head < a.nq + a.nkv;
+        const int64_t at = row + (int64_t)(head - a.nq - (key ? 0 : a.nkv)) * a.head_stride + c * 8;
+        uint8_t* pool = const_cast<uint8_t*>(key ? a.kc : a.vc);
+        if constexpr (FP8) {
+          *reinterpret_cast<uint2*>(pool + at) = pack8_e4m3<DT>(o1);
+          *reinterpret_cast<uint2*>(pool + at + D / 2) = pack8_e4m3<DT>(o2);
+        } else {
+          *reinterpret_cast<uint4*>(pool + 2 * at) = o1;
+          *reinterpret_cast<uint4*>(pool + 2 * (at + D / 2)) = o2;
+        }
       }
     }
   }
@@ -226,7 +256,7 @@ int tsb_paged_kv_store(const TsbPagedCache* cache, const TsbPagedBatch* batch, c
   s.sin = sin;
   s.q_out = static_cast<uint16_t*>(q_out);
   s.max_rope = max_pos;
-  const dim3 grid(batch->n_tokens);
+  const dim3 grid((batch->n_tokens + 256 / kStoreToken - 1) / (256 / kStoreToken));
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   auto go = [&](auto dt, auto d, auto fp8, auto tf) {
     paged_store_kernel<decltype(dt)::value, decltype(d)::value, decltype(fp8)::value, decltype(tf)::value>

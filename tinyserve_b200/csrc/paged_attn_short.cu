@@ -31,7 +31,7 @@ namespace {
 
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
 constexpr int kMaxSeqs = 512;    // sequences of one launch
-constexpr int kMaxCtas = 444;    // three on each SM of a B200
+constexpr int kMaxCtas = 592;    // four on each SM of a B200
 constexpr int kItemCost = 1;     // an item's fixed work in steps
 constexpr int kMinPiece = 16;    // steps: four a warp; joining parts costs as much as five or six
 constexpr int kMaxParts = 64;    // of an item
@@ -53,9 +53,9 @@ template <int D, bool FP8>
 struct Ring {
   static constexpr int kRowBytes = D * (FP8 ? 1 : 2);
   static constexpr int kHalf = step_of<D>() * kRowBytes;
-  static constexpr int kSteps = FP8 ? 4 : 3;
+  static constexpr int kSteps = 3;
   static constexpr int kBytes = kWarps * kSteps * 2 * kHalf;
-  static constexpr int kPerSm = FP8 ? 3 : 2;
+  static constexpr int kPerSm = !FP8 ? 2 : D == 64 ? 4 : 3;
 };
 // Byte of 16-byte chunk c of row r: chunks of a row are exchanged so that the
 // rows and chunks that lanes read together lie in different banks.
