@@ -441,32 +441,51 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows(const SampleArgs a) {
   // ---- the sum of all weights; without filters the race
   double sum;
   {
-    // two floats, so that a row's place in memory does not show in its last bit
-    float part = 0.f, rest = 0.f;
-    // (x - max) * c is enough unless it could be 0 * infinity or infinity - infinity
-    const bool plain = top < INFINITY && inv > 1e-30f && inv < 1e30f;
-    const float c = inv * 1.4426950408889634f;
-    each([&](int i, const float(&v)[PER]) {
-      float d[PER], z[PER];
-      if (!filtered && !by_min && !greedy) noise_of(i, v, z);
+    // Two floats, so that a row's place in memory does not show in its last bit;
+    // from 1 on, so that w is never the larger summand and the rounding of a sum
+    // is what comes out of undoing it.
+    float part = 1.f, rest = 0.f;
+    const auto add = [&](float w) {
+      const float s = part + w;
+      rest += w - (s - part);
+      part = s;
+    };
+    const bool free_race = !filtered && !by_min && !greedy;
+    if (top < INFINITY && inv > 1e-30f && inv < 1e30f) {  // no 0 * infinity, no infinity - infinity
+      const float c = inv * 1.4426950408889634f;
+      each([&](int i, const float(&v)[PER]) {
+        float d[PER], z[PER];
+        if (free_race) noise_of(i, v, z);
 #pragma unroll
-      for (int e = 0; e < PER; ++e) {
-        d[e] = plain ? (v[e] - top) * inv : scaled(v[e]);
-        float w;
-        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(plain ? (v[e] - top) * c : d[e] * 1.4426950408889634f));
-        const float s = part + w, b = s - part;
-        rest += (part - (s - b)) + (w - b);
-        part = s;
-        if (mass_first && v[e] > -INFINITY) put(bin_of(v[e]), w);
-      }
-      if (early) own(i, v);
-      if (!filtered && !by_min && !greedy) {
+        for (int e = 0; e < PER; ++e) {
+          d[e] = fmaxf(v[e] - top, -FLT_MAX);
+          float w;
+          asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(d[e] * c));
+          add(w);
+          if (mass_first && v[e] > -INFINITY) put(bin_of(v[e]), w);
+        }
+        if (early) own(i, v);
+        if (free_race) {
 #pragma unroll
-        for (int e = 0; e < PER; ++e)
-          if (i + e == first || d[e] > -INFINITY) race(i + e, scaled(v[e]), z[e]);
-      }
-    });
-    sum = block_reduce((double)part + (double)rest, [](double q, double r) { return q + r; },
+          for (int e = 0; e < PER; ++e)
+            if (v[e] > -INFINITY) race(i + e, d[e] * inv, z[e]);
+        }
+      });
+    } else {
+      each([&](int i, const float(&v)[PER]) {
+        float z[PER];
+        if (free_race) noise_of(i, v, z);
+#pragma unroll
+        for (int e = 0; e < PER; ++e) {
+          const float d = scaled(v[e]), w = expf(d);
+          add(w);
+          if (mass_first && v[e] > -INFINITY) put(bin_of(v[e]), w);
+          if (free_race && (i + e == first || d > -INFINITY)) race(i + e, d, z[e]);
+        }
+        if (early) own(i, v);
+      });
+    }
+    sum = block_reduce(((double)part - 1.) + (double)rest, [](double q, double r) { return q + r; },
                        reinterpret_cast<double*>(sh.red));
   }
   if (threadIdx.x == 0) sh.sum = sum;
