@@ -21,7 +21,7 @@ namespace {
 // Bound by the bytes of the rows.  A thread takes 8 dims of a head's lower half
 // with the 8 of its upper half (two 16-byte loads, two 16-byte stores), so
 // rotation needs no exchange, for every 32nd (D = 64) or 16th head of its
-// token: the table's values are read once for all of them, and up to four
+// token: the table's values are read once for all of them, and up to three
 // heads' loads are under way together, ahead of the look-ups of sequence and
 // page that the stores wait for.  Products and sums are rounded one by one in
 // fp32 (no contraction), then once to the 16-bit type.
@@ -58,8 +58,12 @@ template <int DT>
 __device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
   uint32_t w[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    w[i] = (uint32_t)from_f32<DT>(x[2 * i]) | ((uint32_t)from_f32<DT>(x[2 * i + 1]) << 16);
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (DT == TSB_DT_F16)
+      asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w[i]) : "f"(x[2 * i + 1]), "f"(x[2 * i]));
+    else
+      asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[i]) : "f"(x[2 * i + 1]), "f"(x[2 * i]));
+  }
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
@@ -84,10 +88,10 @@ __device__ __forceinline__ uint2 pack8_e4m3(uint4 v) {
 }
 
 template <int DT, int D, bool FP8, bool TF32>
-__global__ void __launch_bounds__(256) paged_store_kernel(const StoreArgs s) {
+__global__ void __launch_bounds__(256, 4) paged_store_kernel(const StoreArgs s) {
   const PagedArgs& a = s.p;
   constexpr int kC = D / 16;  // 8-dim chunks of a half
-  constexpr int kSlots = kStoreToken / kC, kAhead = 4;
+  constexpr int kSlots = kStoreToken / kC, kAhead = 3;
   const int token = blockIdx.x * (256 / kStoreToken) + threadIdx.x / kStoreToken;
   if (token >= a.n_tokens) return;
   const int c = threadIdx.x % kC, slot = threadIdx.x % kStoreToken / kC, heads = a.nq + 2 * a.nkv;
