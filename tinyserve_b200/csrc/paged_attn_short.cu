@@ -32,7 +32,7 @@ namespace {
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
 constexpr int kMaxSeqs = 512;    // sequences of one launch
 constexpr int kMaxCtas = 592;    // four on each SM of a B200
-constexpr int kItemCost = 1;     // an item's fixed work in steps
+constexpr int kItemCost = 12;    // a part's fixed work in steps (look-ups, first copies, joining): three a warp
 constexpr int kMinPiece = 16;    // steps: four a warp; joining parts costs as much as five or six
 constexpr int kMaxParts = 64;    // of an item
 constexpr float kGrow = 6.f;
