@@ -36,6 +36,19 @@
 // two that divides the page size), other 16-bit pools by 16-byte asynchronous
 // copies, e4m3 pools through registers, widened on the way.
 //
+// What bounds it: exponentials first (16 a cycle and SM: 122 us for a prompt of
+// 4096 tokens with 64 heads; its products would take 83 us at the measured bf16
+// rate), then what a step costs around them.  Measured there: 266 us, 0.52
+// PFLOP/s, the two tiles' rows 2200 of a step's 3700 cycles in their exponentials,
+// 600 waiting for scores, the rest finding the maximum, masking and handing
+// over.  What decided the time otherwise: 128 keys a step (S, P and O fill
+// tensor memory), code that stays in the instruction caches (loops unrolled to
+// 275 KB took 516 us, rolled 364), S read twice in 32-column pieces (held whole, its 128
+// registers left none to keep exponentials in flight), scores of the next step
+// issued as soon as a row is read.  Exponentials on the multiply-add units for a
+// quarter of the weights made it slower: instructions, not the exponential
+// unit alone, fill a step.
+//
 // A weight of zero times a value that is not finite would be NaN: in tiles
 // where the mask hides something from some row, values that are not finite
 // are replaced by zeros as they are loaded, and rows that do see them get them
@@ -54,7 +67,7 @@ constexpr int kWarpMma = 8, kWarpTma = 9, kWarpQ = 10, kQWarps = 2, kWarpKv = 12
 constexpr int kThreads = 32 * (kWarpKv + kKvWarps);
 enum Feed { kFeedTma, kFeedCopy, kFeedWiden };  // how K and V reach shared memory
 constexpr int kMaxSeqs = 512;   // sequences of one launch
-constexpr int kItemCost = 2;    // an item's fixed work in key tiles
+constexpr int kItemCost = 4;    // an item's fixed work (Q, output) in key tiles; below kMinPiece
 constexpr int kMinPiece = 6;    // a CTA's least share
 constexpr int kMaxCtas = 148;
 constexpr float kGrow = 6.f;    // rescale when the maximum grows by more (log2)

@@ -24,6 +24,12 @@
 // into equal pieces, and an item's last piece joins its parts in key order.
 // The four warps of a CTA take a piece's steps in turn and are joined in
 // shared memory.
+//
+// Measured: 64 tokens over up to 4096 positions, 8 KV heads of 64: 61 us from a
+// bf16 cache (5.0 TB/s, 77% of the measured copy rate), 48 us from an e4m3 one (50%: its
+// conversions and half as many bytes a step leave it bound by instructions);
+// one token over 500 positions 9 us, launch and the chain of look-up, copy,
+// products and joining.
 #include "paged.cuh"
 
 namespace tsb {

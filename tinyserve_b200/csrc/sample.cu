@@ -34,7 +34,10 @@
 // copies its 16-byte pieces ahead into shared memory with a ring of
 // asynchronous copies; held in registers they were waited for when the ring
 // moved on, and loops unrolled over several loads were bound by their own
-// first fetch.
+// first fetch.  Measured (201088 tokens): one fp32 row with top-p 35 us; 32 fp32 rows
+// without filters 34 us (1.5 TB/s of logits and noise); 64 bf16 rows 33 us with
+// min-p, 40 us with top-k, 134 us with top-p, whose warm rows keep more tokens
+// than the lists hold and take two more passes.
 #include <cfloat>
 
 #include "tc05.cuh"
