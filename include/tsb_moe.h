@@ -394,7 +394,7 @@ size_t tsb_paged_workspace(int32_t head_dim);
 
 /* RoPE and cache store of a fused projection's rows: qkv [n_tokens,
  * (n_q_heads + 2 n_kv_heads) * head_dim], rows qkv_stride elements apart; cos
- * / sin [max_pos, head_dim / 2] (table_dtype TSB_DT_F32 or the cache's dtype),
+ * / sin [max_pos, head_dim / 2] (table_dtype TSB_DT_*),
  * halves rotated, the angle of a token's position.  The rotated queries go to
  * q_out [n_tokens, n_q_heads, head_dim]; rotated keys and the values are
  * rounded to dtype and stored in their pages (e4m3: rounded once more, values

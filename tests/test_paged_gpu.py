@@ -229,7 +229,7 @@ def test_in_a_graph(ops):
 
 
 @pytest.mark.parametrize("held", ["same", "e4m3"])
-@pytest.mark.parametrize("tables", ["same", "f32"])
+@pytest.mark.parametrize("tables", ["same", "f32", "other"])
 @pytest.mark.parametrize("dtype", [BF, F16])
 @pytest.mark.parametrize("d", [64, 128])
 def test_store(ops, d, dtype, tables, held):
@@ -243,7 +243,9 @@ def test_store(ops, d, dtype, tables, held):
     wide = torch.randn(b.n, (nq + 2 * nkv) * d + 16, generator=g).to(dtype).cuda()
     qkv = wide[:, :(nq + 2 * nkv) * d]
     ang = torch.arange(400)[:, None] * 10000.0 ** (-torch.arange(0, d, 2) / d)[None, :]
-    cos, sin = (t.to(torch.float32 if tables == "f32" else dtype).cuda() for t in (ang.cos(), ang.sin()))
+    other = F16 if dtype == BF else BF
+    held_in = {"f32": torch.float32, "same": dtype, "other": other}[tables]
+    cos, sin = (t.to(held_in).cuda() for t in (ang.cos(), ang.sin()))
     k0, v0 = b.k.clone(), b.v.clone()
     q = ops.paged_kv_store(qkv, cos, sin, b.k, b.v, b.table, b.cu, b.kv, n_q_heads=nq)
     x = qkv.double().view(b.n, nq + 2 * nkv, d)

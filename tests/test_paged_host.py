@@ -72,7 +72,7 @@ def test_store_refusals():
                                     out, P, 1 << 30, None)
 
     for kw, code in ((dict(qkv=None), 1), (dict(cos=None), 1), (dict(out=None), 1), (dict(stride=632), 1),
-                     (dict(stride=644), 1), (dict(qkv=P + 2), 1), (dict(table=_lib.DT_F16), 2), (dict(nq=0), 1)):
+                     (dict(stride=644), 1), (dict(qkv=P + 2), 1), (dict(table=7), 2), (dict(nq=0), 1)):
         assert store(**kw) == code, kw
 
 

@@ -38,9 +38,9 @@ struct StoreArgs {
   int max_rope;
 };
 
-template <int DT, bool TF32>
+template <int TT>
 __device__ __forceinline__ void load_table8(const void* t, int64_t at, float (&r)[8]) {
-  if constexpr (TF32) {
+  if constexpr (TT == TSB_DT_F32) {
     const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(t) + at);
     const float4 a = p[0], b = p[1];
     r[0] = a.x, r[1] = a.y, r[2] = a.z, r[3] = a.w;
@@ -50,8 +50,8 @@ __device__ __forceinline__ void load_table8(const void* t, int64_t at, float (&r
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      r[2 * i] = to_f32<DT>((uint16_t)w[i]);
-      r[2 * i + 1] = to_f32<DT>((uint16_t)(w[i] >> 16));
+      r[2 * i] = to_f32<TT>((uint16_t)w[i]);
+      r[2 * i + 1] = to_f32<TT>((uint16_t)(w[i] >> 16));
     }
   }
 }
@@ -89,7 +89,7 @@ __device__ __forceinline__ uint2 pack8_e4m3(uint4 v) {
   return make_uint2(o[0], o[1]);
 }
 
-template <int DT, int D, bool FP8, bool TF32>
+template <int DT, int D, bool FP8, int TT>
 __global__ void __launch_bounds__(256, 4) paged_store_kernel(const StoreArgs s) {
   const PagedArgs& a = s.p;
   constexpr int kC = D / 16;  // 8-dim chunks of a half
@@ -120,8 +120,8 @@ __global__ void __launch_bounds__(256, 4) paged_store_kernel(const StoreArgs s) 
     return;
   }
   float cs[8], sn[8];
-  load_table8<DT, TF32>(s.cos, (int64_t)pos * (D / 2) + c * 8, cs);
-  load_table8<DT, TF32>(s.sin, (int64_t)pos * (D / 2) + c * 8, sn);
+  load_table8<TT>(s.cos, (int64_t)pos * (D / 2) + c * 8, cs);
+  load_table8<TT>(s.sin, (int64_t)pos * (D / 2) + c * 8, sn);
   const int64_t row = cached_row(a, b, pos);
   for (int first = slot; first < heads; first += kAhead * kSlots) {
     if (first > slot) load(first);
@@ -247,8 +247,8 @@ int tsb_paged_kv_store(const TsbPagedCache* cache, const TsbPagedBatch* batch, c
   StoreArgs s{};
   const int rc = paged_args(cache, batch, n_q_heads, workspace, workspace_bytes, s.p);
   if (rc) return rc;
-  if (table_dtype != TSB_DT_F32 && table_dtype != cache->dtype)
-    return fail(TSB_ERR_UNSUPPORTED, "cos / sin must be fp32 or the cache's dtype");
+  if (table_dtype != TSB_DT_F32 && table_dtype != TSB_DT_BF16 && table_dtype != TSB_DT_F16)
+    return fail(TSB_ERR_UNSUPPORTED, "cos / sin must be fp32, bf16 or f16");
   if (batch->n_tokens == 0 || batch->n_seqs == 0) return TSB_OK;
   if (!qkv || !cos || !sin || !q_out) return fail(TSB_ERR_INVALID, "null pointer");
   if (qkv_stride < (int64_t)(n_q_heads + 2 * cache->n_kv_heads) * cache->head_dim || qkv_stride % 8)
@@ -264,15 +264,17 @@ int tsb_paged_kv_store(const TsbPagedCache* cache, const TsbPagedBatch* batch, c
   s.max_rope = max_pos;
   const dim3 grid((batch->n_tokens + 256 / kStoreToken - 1) / (256 / kStoreToken));
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  auto go = [&](auto dt, auto d, auto fp8, auto tf) {
-    paged_store_kernel<decltype(dt)::value, decltype(d)::value, decltype(fp8)::value, decltype(tf)::value>
+  auto go = [&](auto dt, auto d, auto fp8, auto tt) {
+    paged_store_kernel<decltype(dt)::value, decltype(d)::value, decltype(fp8)::value, decltype(tt)::value>
         <<<grid, 256, 0, st>>>(s);
   };
   dispatch_paged(*cache, [&](auto dt, auto d, auto fp8) {
     if (table_dtype == TSB_DT_F32)
-      go(dt, d, fp8, std::true_type{});
+      go(dt, d, fp8, std::integral_constant<int, TSB_DT_F32>{});
+    else if (table_dtype == TSB_DT_BF16)
+      go(dt, d, fp8, std::integral_constant<int, TSB_DT_BF16>{});
     else
-      go(dt, d, fp8, std::false_type{});
+      go(dt, d, fp8, std::integral_constant<int, TSB_DT_F16>{});
   });
   return launched();
 }

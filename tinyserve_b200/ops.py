@@ -158,7 +158,7 @@ def paged_kv_store(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_ca
     their pages; returns the rotated queries [N, n_q_heads, D].
 
     qkv         [N, (n_q_heads + 2 kv_heads) * D] bf16 / f16, contiguous rows: the new tokens of all sequences
-    cos, sin    [positions, D / 2] fp32 or qkv's dtype; halves rotated (the GPT-OSS convention)
+    cos, sin    [positions, D / 2] fp32, bf16 or f16; halves rotated (the GPT-OSS convention)
     k_cache, v_cache  [pages, kv_heads, page_size, D] of qkv's dtype or float8_e4m3fn, any strides with a
                 contiguous last dimension; D 64 or 128
     page_table  int32 [B, pages per sequence]
@@ -170,8 +170,8 @@ def paged_kv_store(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_ca
     if qkv.dim() != 2 or qkv.shape[1] != (n_q_heads + 2 * cache.n_kv_heads) * d or (n and qkv.stride(1) != 1):
         raise ValueError("qkv must be [tokens, (n_q_heads + 2 kv_heads) * head_dim] with contiguous rows")
     if (cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != sin.dtype or cos.shape[1] * 2 != d
-            or cos.dtype not in (torch.float32, qkv.dtype) or not cos.is_contiguous() or not sin.is_contiguous()):
-        raise ValueError("cos and sin must be contiguous [positions, head_dim / 2] of fp32 or qkv's dtype")
+            or cos.dtype not in _DT or not cos.is_contiguous() or not sin.is_contiguous()):
+        raise ValueError("cos and sin must be contiguous [positions, head_dim / 2] of fp32, bf16 or f16")
     _require_cuda(cos, sin, q_out)
     if q_out is None:
         q_out = torch.empty(n, n_q_heads, d, dtype=qkv.dtype, device=qkv.device)
