@@ -35,8 +35,8 @@
 // asynchronous copies; held in registers they were waited for when the ring
 // moved on, and loops unrolled over several loads were bound by their own
 // first fetch.  Measured (201088 tokens): one fp32 row with top-p 35 us; 32 fp32 rows
-// without filters 34 us (1.5 TB/s of logits and noise); 64 bf16 rows 33 us with
-// min-p, 40 us with top-k, 134 us with top-p, whose warm rows keep more tokens
+// without filters 30 us (1.7 TB/s of logits and noise); 64 bf16 rows 33 us with
+// min-p, 41 us with top-k, 112 us with top-p, whose warm rows keep more tokens
 // than the lists hold and take two more passes.
 #include <cfloat>
 
@@ -297,6 +297,13 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows(const SampleArgs a) {
     win = more(win, key_of(r, i));
   };
 
+  // The warp's lanes learn of each other's best races, one distance a call.
+  int apart = 1;
+  const auto share_ahead = [&] {
+    ahead = fmaxf(ahead, __shfl_xor_sync(0xffffffffu, ahead, apart));
+    apart = apart == 16 ? 1 : 2 * apart;
+  };
+
   // ---- histograms: of the whole row by distance, or of one bin by keys
   uint64_t key_hi = 0;
   int level = 0, shift = 0, whole_bin = 0;
@@ -472,6 +479,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows(const SampleArgs a) {
 #pragma unroll
           for (int e = 0; e < PER; ++e)
             if (v[e] > -INFINITY) race(i + e, d[e] * inv, z[e]);
+          share_ahead();
         }
       });
     } else {
@@ -542,7 +550,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows(const SampleArgs a) {
       if (!listed && sh.bin >= 0 && sh.bin < kBins - 1) {
         // lists of what may be kept; where that is too much, of the bin alone
         cut = top - (sh.bin + 1.5f) / kPerUnit - slack;
-        for (int only = 0; only < 2 && !listed && cut < top && cut > -INFINITY; ++only) {
+        const bool many = sh.before_count + sh.bin_count > (uint32_t)(kOwn * kWarps / 2 * ctas);
+        for (int only = many; only < 2 && !listed && cut < top && cut > -INFINITY; ++only) {
           if (only) cap = fminf(top, top - (sh.bin - 0.5f) / kPerUnit + slack);
           owned = 0;
           each(own);
@@ -658,6 +667,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows(const SampleArgs a) {
         const bool kept = v[e] > floor_x || (v[e] == floor_x && key_of(v[e], i + e) >= threshold);
         if (i + e == first || (kept && d > -INFINITY && (least <= 0.f || expf(d) >= least))) race(i + e, d, z[e]);
       }
+      share_ahead();
     });
   }
   if (!greedy) win = block_reduce(win, more, sh.red);
