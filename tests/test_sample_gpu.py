@@ -187,3 +187,17 @@ def test_refusals(ops):
             f()
     tok, lp = ops.sample_tokens(x[:0], e[:0])
     assert tok.shape == lp.shape == (0,)
+
+
+@pytest.mark.parametrize("likely", [6000, 9000])
+@pytest.mark.parametrize("rows", [1, 2, 40])
+def test_likely_tokens_side_by_side(ops, rows, likely):
+    """What top-p (or a large k) keeps lies in neighbouring tokens, so that few
+    warps of a cluster's CTAs hold all of it: their first lists overflow and
+    the bin of the limit is collected alone."""
+    x, e = inputs(rows, 201088, torch.float32, rows + likely, spread=0.3)
+    x[:, 70000:70000 + likely] += 12.0
+    p = np.linspace(0.5, 0.95, rows).astype(np.float32)
+    check(*both(ops, x, e, None, None, p, None))
+    k = np.full(rows, 2000, np.int32)
+    check(*both(ops, x, e, None, k, p, None))

@@ -82,7 +82,8 @@ struct Shared {
   float own[kWarps][kOwn];
   uint64_t red[kWarps], red2[kWarps];
   // read by the other CTAs
-  uint64_t best, race, low, result_key, result_mass, owned;
+  uint64_t best, race, low, result_key, result_mass;
+  uint64_t owned[2];  // taken in turn
   double sum;
   // the bin that a scan found
   int bin;
@@ -346,11 +347,17 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows(const SampleArgs a) {
       owned += __popc(all);
     }
   };
-  const auto agree = [&] {  // whether every list of the cluster holds its tokens
+  // Whether every list of the cluster holds its tokens.  Two calls may follow
+  // each other with no barrier between one's reads and the other's write, so they
+  // take two words in turn: a word is written again after the barrier of the call
+  // in between, which nobody passes before everyone has read it.
+  int turn = 0;
+  const auto agree = [&] {
     const uint64_t most = block_reduce((uint64_t)owned, more, sh.red);
-    if (threadIdx.x == 0) sh.owned = most;
+    if (threadIdx.x == 0) sh.owned[turn] = most;
     sync_all();
-    listed = of_cluster(&sh.owned, more) <= kOwn;
+    listed = of_cluster(&sh.owned[turn], more) <= kOwn;
+    turn ^= 1;
   };
   const auto visit = [&](auto f) {  // f(index, logit) of the lists, or of the row
     if (listed) {
