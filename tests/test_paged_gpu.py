@@ -406,3 +406,56 @@ def test_refusals(ops):
         more = {"q_out": a.pop("q_out")} if "q_out" in a else {}
         with pytest.raises(ValueError):
             ops.paged_kv_store(a["qkv"], a["cos"], a["sin"], b.k, b.v, b.table, b.cu, b.kv, n_q_heads=8, **more)
+
+
+def padded(b, rows):
+    """q and out with ``rows`` rows, those past the batch's own of no sequence."""
+    q = torch.zeros(rows, b.nq, b.d, dtype=b.dtype, device="cuda")
+    q[:b.n] = b.q
+    return q, torch.full_like(q, 7.0)
+
+
+@pytest.mark.parametrize("held", [BF, E4])
+@pytest.mark.parametrize("q_lens,most", [([8, 1], 8), ([2], 64), ([32, 1], 32), ([3, 0, 40, 2], 40), ([1, 1, 1], 5)])
+def test_buffer_of_full_length_for_every_sequence(ops, q_lens, most, held):
+    """As many rows as n_seqs sequences of max_q new tokens need, of which the
+    sequences at hand take fewer: every one of theirs is served."""
+    b = R.Batch(q_lens, [90 + 7 * i for i in range(len(q_lens))], 8, 1, 64, 16, BF, held, seed=most)
+    q, out = padded(b, most * len(q_lens))
+    ops.paged_attention(q, b.k, b.v, b.table, b.cu, b.kv, most, sinks=b.sinks, out=out)
+    check(out[:b.n], b)
+    assert (out[b.n:] == 7.0).all()
+
+
+def test_graph_of_full_sequences_replayed_with_shorter_ones(ops):
+    """Captured with every sequence at its longest, replayed with other cu_q."""
+    full = R.Batch([32, 32], [100, 70], 8, 1, 64, 16, BF, BF, seed=1)
+    less = R.Batch([31, 2], [95, 66], 8, 1, 64, 16, BF, BF, seed=2)
+    pool = max(full.k.shape[0], less.k.shape[0])
+    for t in (full, less):
+        for n in ("k", "v"):
+            grown = torch.zeros(pool, 1, 16, 64, dtype=BF, device="cuda")
+            grown[:getattr(t, n).shape[0]] = getattr(t, n)
+            setattr(t, n, grown)
+        table = torch.full((2, 8), -1, dtype=torch.int32, device="cuda")
+        table[:, :t.table.shape[1]] = t.table
+        t.table = table
+    q, out = padded(full, 64)
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        ops.paged_attention(q, full.k, full.v, full.table, full.cu, full.kv, 32, sinks=full.sinks, out=out)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=st):
+            ops.paged_attention(q, full.k, full.v, full.table, full.cu, full.kv, 32, sinks=full.sinks, out=out)
+        g.replay()
+        st.synchronize()
+        check(out, full)
+        for n in ("k", "v", "kv", "table", "sinks", "cu"):
+            getattr(full, n).copy_(getattr(less, n))
+        q[:less.n] = less.q
+        out.fill_(7.0)
+        g.replay()
+        st.synchronize()
+    check(out[:less.n], less)
+    assert (out[less.n:] == 7.0).all()

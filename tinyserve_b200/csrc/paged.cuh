@@ -102,10 +102,12 @@ struct AttnCall {
   float* part;         // partial results of split key ranges
   float scale;
   int window, keep_first;  // keep_first is 0 without a window
+  int short_rows;          // the long kernel leaves sequences with at most so many rows per KV head to the short one
 };
 
 // A sequence with at most this many rows (new tokens x query heads of a KV
-// head) per KV head goes to the short kernel, one with more to the long one.
+// head) per KV head goes to the short kernel, one with more to the long one
+// (which takes all where there is no launch of the short one).
 constexpr int kShortRows = 16;
 
 // Workspace: the error word, the counters, the partial results.

@@ -1,5 +1,5 @@
 // Attention of prompt chunks over a paged KV cache on the tensor cores
-// (sequences with more than kShortRows rows per KV head; tsb_paged_attention).
+// (sequences with more than short_rows rows per KV head; tsb_paged_attention).
 //
 // Rows: the query heads of a KV head share its keys, so a sequence's rows for
 // one KV head are (token, head of the group), token-major; 256 of them, two
@@ -145,7 +145,7 @@ __device__ __forceinline__ Range key_tiles(const AttnCall& c, int q_len, int kv_
 }
 __device__ __forceinline__ int tiles_of(const AttnCall& c, int q_len) {
   const int rows = q_len * c.p.G;
-  return rows > kShortRows ? (rows + kItemRows - 1) / kItemRows : 0;
+  return rows > c.short_rows ? (rows + kItemRows - 1) / kItemRows : 0;
 }
 // Every row with a position in [p0, p1] sees all keys of the tile at j0.
 __device__ __forceinline__ bool open_tile(const AttnCall& c, int p0, int p1, int j0) {
