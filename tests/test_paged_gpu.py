@@ -459,3 +459,20 @@ def test_graph_of_full_sequences_replayed_with_shorter_ones(ops):
         st.synchronize()
     check(out[:less.n], less)
     assert (out[less.n:] == 7.0).all()
+
+
+def test_rows_that_overlap_are_refused(ops):
+    """qkv rows that share memory (an expanded row, a window sliding over a
+    vector) do not hold what the operator would read behind the first."""
+    b = R.Batch([3], [5], 8, 2, 64, 16, BF, BF)
+    t = torch.rand(8, 32, device="cuda")
+    width = 12 * 64
+    row = torch.zeros(width + 16, dtype=BF, device="cuda")
+    for qkv in (row[:width].expand(3, width), row.as_strided((3, width), (8, 1))):
+        with pytest.raises(RuntimeError, match="overlap"):
+            ops.paged_kv_store(qkv, t, t, b.k, b.v, b.table, b.cu, b.kv, n_q_heads=8)
+    b = R.Batch([1], [5], 8, 2, 64, 16, BF, BF)
+    one = torch.randn(1, width, device="cuda").to(BF)
+    want = ops.paged_kv_store(one, t, t, b.k, b.v, b.table, b.cu, b.kv, n_q_heads=8)
+    got = ops.paged_kv_store(one.as_strided((1, width), (0, 1)), t, t, b.k, b.v, b.table, b.cu, b.kv, n_q_heads=8)
+    assert torch.equal(got, want)  # the stride of a single row says nothing

@@ -179,8 +179,9 @@ def paged_kv_store(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_ca
         raise ValueError("q_out must be contiguous [tokens, n_q_heads, head_dim] of qkv's dtype")
     stream = _stream_of(qkv)
     ws = _paged_workspace(qkv.device, d, stream) if workspace is None else workspace
+    row = qkv.stride(0) if n > 1 else qkv.shape[1]
     _lib.check(_lib.lib().tsb_paged_kv_store(
-        ctypes.byref(cache), ctypes.byref(batch), qkv.data_ptr(), max(qkv.stride(0), qkv.shape[1]), n_q_heads,
+        ctypes.byref(cache), ctypes.byref(batch), qkv.data_ptr(), row, n_q_heads,
         cos.data_ptr(), sin.data_ptr(), _DT[cos.dtype], cos.shape[0], q_out.data_ptr(), ws.data_ptr(), ws.numel(),
         stream))
     return q_out
