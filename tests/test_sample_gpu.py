@@ -201,3 +201,28 @@ def test_likely_tokens_side_by_side(ops, rows, likely):
     check(*both(ops, x, e, None, None, p, None))
     k = np.full(rows, 2000, np.int32)
     check(*both(ops, x, e, None, k, p, None))
+
+
+@pytest.mark.parametrize("best,level", [(100, 30000), (5000, 1000), (3000, 3000)])
+def test_top_p_that_ends_with_a_level(ops, best, level):
+    """Three levels of equal logits, top-p within a few roundings of the mass of
+    the first two: no more than the first token or so of the last level is
+    kept, and none of the better ones is lost."""
+    rows, vocab = 160, 60000  # one CTA a row
+    x = torch.full((rows, vocab), -30.0, device="cuda")
+    e = torch.ones(rows, vocab, device="cuda")
+    a = torch.linspace(0.3, 3.0, rows, dtype=torch.float64).float().cuda()
+    x[:, :best] = 0.0
+    x[:, best:best + level] = -a[:, None]
+    tail = slice(best + level, best + level + 2000)
+    x[:, tail] = -2.0 * a[:, None]
+    w = torch.exp(x.double())
+    limit = (w[:, :best + level].sum(1) / w.sum(1)).cpu().numpy()
+    e[:, best + level + 1000] = 1e-12  # in the middle of the last level: would win if kept
+    e[:, 7] = 1e-6                     # of the best level: wins
+    for ulps in range(-3, 4):
+        p = limit.astype(np.float32)
+        for _ in range(abs(ulps)):
+            p = np.nextafter(p, np.float32(2.0 if ulps > 0 else 0.0))
+        tok, _ = ops.sample_tokens(x, e, top_p=torch.from_numpy(p).cuda())
+        assert (tok == 7).all(), (ulps, tok[tok != 7][:5])
