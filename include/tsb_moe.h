@@ -387,10 +387,17 @@ typedef struct {
   int32_t n_seqs, n_tokens, max_q;
 } TsbPagedBatch;
 
-/* Workspace of the two paged entry points, 256-byte aligned, zero-initialised
- * once; one workspace serves successive calls on a stream (any batch).
- * tsb_read_device_error(workspace, ...) reads its error word. */
+/* Workspace of the two paged entry points, 256-byte aligned, its first
+ * TSB_PAGED_ZEROED bytes zero-initialised once; one workspace serves successive
+ * calls on a stream (any batch).  Graphs that may run at the same time need one
+ * each.  tsb_read_device_error(workspace, ...) reads its error word. */
+#define TSB_PAGED_ZEROED 65536
 size_t tsb_paged_workspace(int32_t head_dim);
+
+/* The graph capture that `stream` is in: its number, 0 when it is in none.  What
+ * a call inside one writes is written when the graph runs, so scratch that is
+ * first zeroed there belongs to that graph. */
+int tsb_capture_id(void* stream, uint64_t* id);
 
 /* RoPE and cache store of a fused projection's rows: qkv [n_tokens,
  * (n_q_heads + 2 n_kv_heads) * head_dim], rows qkv_stride elements apart; cos

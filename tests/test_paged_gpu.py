@@ -476,3 +476,71 @@ def test_rows_that_overlap_are_refused(ops):
     want = ops.paged_kv_store(one, t, t, b.k, b.v, b.table, b.cu, b.kv, n_q_heads=8)
     got = ops.paged_kv_store(one.as_strided((1, width), (0, 1)), t, t, b.k, b.v, b.table, b.cu, b.kv, n_q_heads=8)
     assert torch.equal(got, want)  # the stride of a single row says nothing
+
+
+def captured(f, pool=None):
+    """A graph of f() on the capture stream that all such graphs share, without a warm-up there."""
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, pool=pool):
+        out = f()
+    return g, out
+
+
+def test_first_calls_inside_captures(ops):
+    """Graphs captured on a stream that has run no paged operator: each holds its
+    own scratch, so the second may run before the first, beside it, or
+    without it, and calls outside any graph are not touched by either."""
+    a = R.Batch([1, 2], [3000, 2000], 8, 1, 64, 16, BF, BF, seed=1)  # both are divided and joined
+    b = R.Batch([1, 30], [2500, 2100], 8, 1, 64, 16, BF, BF, seed=2)
+    want = [attend(ops, t) for t in (a, b)]
+    # memory that is not zero where the graphs take theirs; they run one by one
+    g0, junk = captured(lambda: torch.full((64 << 20,), 0x5A, dtype=torch.uint8, device="cuda"))
+    del junk
+    a_out, b_out = torch.empty_like(a.q), torch.empty_like(b.q)
+    ga, _ = captured(lambda: attend(ops, a, out=a_out), g0.pool())
+    gb, _ = captured(lambda: attend(ops, b, out=b_out), g0.pool())
+    for order in ((gb, ga), (ga, gb)):
+        for g in order:
+            g0.replay(), g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(a_out, want[0]) and torch.equal(b_out, want[1])
+    # with memory of their own they may overlap
+    ga, out_a = captured(lambda: attend(ops, a))
+    gb, out_b = captured(lambda: attend(ops, b))
+    for _ in range(2):
+        gb.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out_b, want[1])
+    ga.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out_a, want[0])
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(20):
+        out_a.fill_(7.0), out_b.fill_(7.0)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(s1):
+            ga.replay()
+        with torch.cuda.stream(s2):
+            gb.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out_a, want[0]) and torch.equal(out_b, want[1])
+    assert torch.equal(attend(ops, a), want[0])
+    qkv = torch.randn(31, 10 * 64, device="cuda").to(BF)
+    t = torch.rand(2500, 32, device="cuda")
+    q = ops.paged_kv_store(qkv, t, t, b.k, b.v, b.table, b.cu, b.kv, n_q_heads=8)
+    gs, out = captured(lambda: ops.paged_kv_store(qkv, t, t, b.k, b.v, b.table, b.cu, b.kv, n_q_heads=8))
+    gs.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, q)
+
+
+def test_errors_inside_captures_are_read(ops):
+    """A graph without a workspace of its own reports to the error word that paged_device_error reads."""
+    b = R.Batch([1, 2], [50, 60], 8, 1, 64, 16, BF, BF)
+    g, _ = captured(lambda: attend(ops, b))
+    g.replay()
+    assert ops.paged_device_error() == 0
+    b.table[1, 1] = b.k.shape[0]
+    g.replay()
+    assert ops.paged_device_error() == 2
+    assert ops.paged_device_error() == 0

@@ -35,7 +35,7 @@ EXPORTS = (
     "tsb_ep_moe_prefill", "tsb_gqa_decode_workspace", "tsb_gqa_decode_attention", "tsb_add_rmsnorm",
     "tsb_gemv_bf16", "tsb_norm_gemv_bf16", "tsb_gemv_bf16_residual", "tsb_gqa_decode_batch_workspace",
     "tsb_gqa_decode_attention_batch", "tsb_norm_qkv_attention",
-    "tsb_paged_workspace", "tsb_paged_kv_store", "tsb_paged_attention", "tsb_sample",
+    "tsb_paged_workspace", "tsb_capture_id", "tsb_paged_kv_store", "tsb_paged_attention", "tsb_sample",
 )
 
 
@@ -127,6 +127,7 @@ def _declare(L: ctypes.CDLL) -> None:
     pc, pb = ctypes.POINTER(TsbPagedCache), ctypes.POINTER(TsbPagedBatch)
     L.tsb_paged_workspace.argtypes = [_i32]
     L.tsb_paged_workspace.restype = _sz
+    L.tsb_capture_id.argtypes = [_vp, ctypes.POINTER(ctypes.c_uint64)]
     L.tsb_paged_kv_store.argtypes = [pc, pb, _vp, _i64, _i32, _vp, _vp, _i32, _i32, _vp, _vp, _sz, _vp]
     L.tsb_paged_attention.argtypes = [pc, pb, _vp, _i64, _i64, _i32, _i32, _i32, _vp, ctypes.c_float, _vp, _vp, _sz,
                                       _vp]

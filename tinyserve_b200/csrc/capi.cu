@@ -337,6 +337,19 @@ int tsb_read_device_error(void* workspace, int32_t* code, void* stream) {
   return TSB_OK;
 }
 
+int tsb_capture_id(void* stream, uint64_t* id) {
+  if (!id) return set_error(TSB_ERR_INVALID, "null pointer");
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long number = 0;
+  const cudaError_t e = cudaStreamGetCaptureInfo(static_cast<cudaStream_t>(stream), &status, &number);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return set_error(TSB_ERR_CUDA, cudaGetErrorString(e));
+  }
+  *id = status == cudaStreamCaptureStatusNone ? 0 : number;
+  return TSB_OK;
+}
+
 int tsb_moe_route(const TsbMoeSpec* spec, const void* x, int32_t T, const void* router_w, const float* router_b,
                   int32_t* ids, float* weights, void* stream) {
   if (!spec) return set_error(TSB_ERR_INVALID, "null pointer");

@@ -111,7 +111,7 @@ struct AttnCall {
 constexpr int kShortRows = 16;
 
 // Workspace: the error word, the counters, the partial results.
-constexpr size_t kPagedHead = 64 * 1024;
+constexpr size_t kPagedHead = TSB_PAGED_ZEROED;  // of the first two; the last are written before they are read
 size_t long_partial_bytes(int head_dim);
 size_t short_partial_bytes(int head_dim);
 int launch_paged_short(const TsbPagedCache& cache, const AttnCall& c, cudaStream_t st);

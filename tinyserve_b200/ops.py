@@ -72,25 +72,41 @@ def weight_bytes(fmt: int, rows: int, cols: int) -> tuple[int, int]:
 # serving step (tinyserve/paged_kv_cache.py:20-122; sliding window with
 # visible first tokens, tinyserve/static_kv_cache.py:282-389).
 # ---------------------------------------------------------------------------
-_paged_ws: dict[tuple[int, int, int], torch.Tensor] = {}
+_paged_ws: dict[tuple[int, int, int], torch.Tensor] = {}                   # by device, head size, stream
+_captured_ws: dict[tuple[int, int, int], tuple[int, torch.Tensor]] = {}    # of the capture that is under way there
+_PAGED_ZEROED = 64 * 1024  # TSB_PAGED_ZEROED
 
 
 def paged_workspace(device: torch.device, head_dim: int) -> torch.Tensor:
     """Zero-initialised scratch of the paged operators.  One workspace serves
     successive calls on one stream; the operators keep one per (device,
-    stream) unless they are given another."""
+    stream) unless they are given another.  A graph captured on a stream where
+    they keep none holds scratch of its own."""
     n = _lib.lib().tsb_paged_workspace(head_dim)
     if n == 0:
         raise RuntimeError("head_dim must be 64 or 128")
-    return torch.zeros(n, dtype=torch.uint8, device=device)
+    ws = torch.empty(n, dtype=torch.uint8, device=device)
+    ws[:_PAGED_ZEROED].zero_()
+    return ws
 
 
 def _paged_workspace(device: torch.device, head_dim: int, stream: int) -> torch.Tensor:
     key = (device.index, head_dim, stream)
     ws = _paged_ws.get(key)
-    if ws is None:
+    if ws is not None:
+        return ws
+    capture = ctypes.c_uint64()
+    _lib.check(_lib.lib().tsb_capture_id(stream, ctypes.byref(capture)))
+    if capture.value == 0:
         ws = _paged_ws[key] = paged_workspace(device, head_dim)
-    return ws
+        return ws
+    # Memory of the graph's, zeroed where the graph runs: nothing outside it may
+    # go by it, and another capture on this stream takes its own.
+    held = _captured_ws.get(key)
+    if held is None or held[0] != capture.value:
+        _captured_ws.pop(key, None)
+        held = _captured_ws[key] = (capture.value, paged_workspace(device, head_dim))
+    return held[1]
 
 
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
@@ -103,12 +119,14 @@ def _stream_of(t: torch.Tensor) -> int:
 
 def paged_device_error(workspace: torch.Tensor | None = None, device: torch.device | None = None) -> int:
     """Read and clear the device error word of a workspace, or of every
-    workspace the paged operators keep for ``device``: 0 when the batches were
+    workspace the paged operators keep for ``device`` (of a stream's graphs with
+    scratch of their own, the last captured one's): 0 when the batches were
     consistent, 2 when one named a page outside the pool or a length beyond
     its table.  Synchronises."""
     if workspace is None:
         device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
-        held = [ws for key, ws in _paged_ws.items() if key[0] == (device.index or 0)]
+        kept = list(_paged_ws.items()) + [(key, ws) for key, (_, ws) in _captured_ws.items()]
+        held = [ws for key, ws in kept if key[0] == (device.index or 0)]
     else:
         held = [workspace]
     code = 0
