@@ -544,3 +544,15 @@ def test_errors_inside_captures_are_read(ops):
     g.replay()
     assert ops.paged_device_error() == 2
     assert ops.paged_device_error() == 0
+
+
+@pytest.mark.parametrize("window,keep", [(2 ** 31 - 1, 0), (2 ** 31 - 1, 2 ** 31 - 1), (60, 2 ** 31 - 1), (60, 2 ** 31 - 100),
+                                         (511, 3), (512, 3), (2000, 5)])
+@pytest.mark.parametrize("held", [BF, E4])
+def test_windows_and_first_tokens_of_any_size(ops, window, keep, held):
+    """Windows and first tokens up to the integers' end, around the table's
+    positions, with rows before the first position."""
+    for lens in (RAGGED, ([300, 8], [450, 5]), ([1, 2], [500, 1])):
+        b = R.Batch(*lens, 8, 1, 64, 16, BF, held, seed=7)
+        kw = dict(window=window, keep_first=keep)
+        check(attend(ops, b, **kw), b, **kw)

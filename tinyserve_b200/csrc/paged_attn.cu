@@ -299,8 +299,10 @@ int tsb_paged_attention(const TsbPagedCache* cache, const TsbPagedBatch* batch, 
   c.q_head_stride = q_head_stride;
   c.sinks = sinks;
   c.scale = scale;
-  c.window = window;
-  c.keep_first = window > 0 ? keep_first : 0;
+  // No position is beyond the table's: a window that covers them all is none, and
+  // what is left of either number stays far from the integers' end.
+  c.window = window < c.p.max_pos ? window : 0;
+  c.keep_first = c.window > 0 ? min(keep_first, c.p.max_pos) : 0;
   c.counters = static_cast<unsigned*>(workspace) + 64;
   c.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + kPagedHead);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
