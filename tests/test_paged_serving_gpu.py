@@ -165,3 +165,19 @@ def test_eos_and_refusals(lm):
             bad()
     with pytest.raises(RuntimeError, match="pages"):
         eng.pool.take(41)
+
+
+def test_steps_of_any_size_take_no_more_memory(lm):
+    """Steps of 40 to 17 tokens, then of 16 to 1, after one of the largest: the
+    scratch of the expert layers does not grow with the sizes met."""
+    eng = engine(lm, chunk_tokens=40, keep_logits=False)
+
+    def serve(n):
+        eng.submit(prompts((n,))[0], 1)
+        eng.run()
+        torch.cuda.synchronize()
+        return torch.cuda.memory_allocated()
+
+    serve(40)
+    few = serve(16)
+    assert all(serve(n) <= few + (1 << 20) for n in [*range(39, 16, -1), *range(15, 0, -1)])

@@ -14,9 +14,11 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
-from .formats import TSB_MXFP4
+from .formats import DENSE, TSB_MXFP4
 
 ACTIVATIONS = {"silu": _lib.ACT_SILU, "swiglu_oai": _lib.ACT_SWIGLU_OAI}
+# Most tokens that tsb_moe_decode runs one by one; more take the grouped path.
+ONE_BY_ONE = 16
 LAYOUTS = {"separate": _lib.GU_SEPARATE, "interleaved": _lib.GU_INTERLEAVED, "chunked": _lib.GU_CHUNKED}
 
 
@@ -98,23 +100,35 @@ class QuantMoE:
             return L.tsb_moe_decode_packed, (spec, self._packed.data_ptr(), self._table.data_ptr())
         return L.tsb_moe_decode, (spec, self._table.data_ptr())
 
+    def workspace_bytes(self, T: int) -> int:
+        """Scratch that :meth:`decode` needs for T tokens."""
+        L = _lib.lib()
+        ws_fn = L.tsb_moe_decode_packed_workspace if self._packed is not None else L.tsb_moe_decode_workspace
+        return ws_fn(ctypes.byref(self.spec), T)
+
     def workspace(self, T: int) -> torch.Tensor:
+        """The layer's own scratch for T tokens, kept from call to call.  Up to
+        ``ONE_BY_ONE`` tokens run one after the other in the same one."""
+        if T <= ONE_BY_ONE and not self.dense:
+            T = 1
         if T not in self._ws_cache:
-            L = _lib.lib()
-            ws_fn = L.tsb_moe_decode_packed_workspace if self._packed is not None else L.tsb_moe_decode_workspace
-            n = ws_fn(ctypes.byref(self.spec), T)
-            self._ws_cache[T] = torch.zeros(n, dtype=torch.uint8, device=self.device)
+            self._ws_cache[T] = torch.zeros(self.workspace_bytes(T), dtype=torch.uint8, device=self.device)
         return self._ws_cache[T]
 
     def decode(self, x: torch.Tensor, ids: torch.Tensor | None = None, weights: torch.Tensor | None = None,
-               out: torch.Tensor | None = None, out_dtype: torch.dtype = torch.bfloat16):
+               out: torch.Tensor | None = None, out_dtype: torch.dtype = torch.bfloat16,
+               workspace: torch.Tensor | None = None):
         """T tokens through the layer.  x: bf16 [T, H] ([1, H] for batch-1
         decode; up to 16 tokens run the batch-1 path per token, more the
         grouped path, each routed expert read once for all its tokens).  With a
         router, returns (out, ids, weights) where ids / weights are the routing
         it chose; without one, ``ids`` (int32 [T, k]) and ``weights`` (fp32
         [T, k]) are inputs.  ``out_dtype`` bf16 (default) or float32 (the
-        unrounded combine; a given ``out`` decides by its own dtype)."""
+        unrounded combine; a given ``out`` decides by its own dtype).
+        ``workspace``: uint8 scratch of at least ``workspace_bytes(T)`` bytes,
+        zeroed once, instead of the layer's own for this T; for more than
+        ``ONE_BY_ONE`` tokens, whose sizes vary: one serves every such T of
+        every quantised (or of every dense) layer on a stream."""
         if x.dtype != torch.bfloat16:
             raise TypeError("x must be bfloat16")
         x = x.contiguous()
@@ -132,7 +146,12 @@ class QuantMoE:
             out = torch.empty(T, self.hidden, dtype=out_dtype, device=self.device)
         if out.dtype not in (torch.bfloat16, torch.float32):
             raise TypeError("out must be bfloat16 or float32")
-        ws = self.workspace(T)
+        if workspace is None or T <= ONE_BY_ONE:
+            ws = self.workspace(T)
+        else:
+            ws = workspace
+            if ws.dtype != torch.uint8 or ws.device != self.device or not ws.is_contiguous():
+                raise ValueError("workspace must be contiguous uint8 on the layer's device")
         fn, lead = self._decode_call(out.dtype == torch.float32)
         rc = fn(
             *lead, x.data_ptr(), T,
@@ -224,6 +243,11 @@ class QuantMoE:
         _lib.check(_lib.lib().tsb_read_device_error(ws.data_ptr(), ctypes.byref(code),
                                                     torch.cuda.current_stream(self.device).cuda_stream))
         return code.value
+
+    @property
+    def dense(self) -> bool:
+        """True when the experts are float tensors."""
+        return self.spec.fmt_gate_up in DENSE
 
     @property
     def is_mxfp4(self) -> bool:

@@ -21,6 +21,7 @@ import torch.nn.functional as F
 
 from . import ops
 from .gptoss import GptOssDecoder
+from .moe import ONE_BY_ONE
 
 
 class PagePool:
@@ -93,6 +94,12 @@ class PagedServingEngine:
         self.sin = (freqs.sin() * rot.attention_scaling).to(torch.bfloat16)
         self.max_batch, self.max_seq, self.chunk_tokens = max_batch, max_seq, chunk_tokens
         self.pool = PagePool(d.L, pages, d.nkv, page_size, d.D, kv_dtype, d.device)
+        # the expert layers' scratch for a step of any size; they run one after the other and share it
+        need = {False: 0, True: 0}  # by QuantMoE.dense
+        for lay in d.layers:
+            moe = lay["moe"]
+            need[moe.dense] = max([need[moe.dense]] + [moe.workspace_bytes(t) for t in range(ONE_BY_ONE + 1, chunk_tokens + 1)])
+        self._expert_ws = {k: torch.zeros(n, dtype=torch.uint8, device=d.device) for k, n in need.items()}
         self.eos = eos_token_id
         self.keep_logits = keep_logits
         self._ids = itertools.count()
@@ -168,7 +175,8 @@ class PagedServingEngine:
             a = ops.paged_attention(q, pool.k[li], pool.v[li], pages, cu, kv, max_q, scale=d.scale,
                                     window=d.window if d.sliding[li] else 0, sinks=lay["sinks"])
             d._norm(x, F.linear(a.view(a.shape[0], -1), lay["wo"], lay["bo"]), lay["ln2"], h)
-            y, _, _ = lay["moe"].decode(h, out_dtype=torch.float32)
+            moe = lay["moe"]
+            y, _, _ = moe.decode(h, out_dtype=torch.float32, workspace=self._expert_ws[moe.dense])
             d._norm(x, y, d._next_norm(li), h)
         return h.index_select(0, (cu[1:] - 1).long())
 
