@@ -1,0 +1,55 @@
+"""The paged serving engine's bookkeeping around a stand-in for the model (no GPU)."""
+from __future__ import annotations
+
+import itertools
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+from tinyserve_b200 import paged
+
+VOCAB, HIDDEN = 32, 8
+
+
+@pytest.fixture
+def engine(monkeypatch):
+    """An engine whose forward pass gives zeros and whose sampler gives the
+    tokens of ``script`` (a list per call), recording what is fed."""
+    eng = paged.PagedServingEngine.__new__(paged.PagedServingEngine)
+    eng.dec = SimpleNamespace(lm_head=torch.zeros(VOCAB, HIDDEN, dtype=torch.bfloat16), device=torch.device("cpu"),
+                              embed=torch.zeros(VOCAB, HIDDEN, dtype=torch.bfloat16), layers=[])
+    eng.max_batch, eng.max_seq, eng.chunk_tokens = 4, 64, 16
+    eng.pool = paged.PagePool(1, 20, 1, 4, 64, torch.bfloat16, torch.device("cpu"))
+    eng.eos, eng.keep_logits = None, False
+    eng._ids, eng._rng = itertools.count(), torch.Generator()
+    eng.waiting, eng.running, eng.finished = [], [], {}
+    eng.fed, eng.script = [], []
+
+    def forward(batch):
+        eng.fed.append([list(ids) for _, ids in batch])
+        assert all(0 <= t < VOCAB for _, ids in batch for t in ids)
+        return torch.zeros(len(batch), HIDDEN, dtype=torch.bfloat16)
+
+    def sample(logits, noise=None, **kw):
+        tokens = eng.script.pop(0) if eng.script else [1] * logits.shape[0]
+        assert len(tokens) == logits.shape[0]
+        return torch.tensor(tokens), torch.zeros(len(tokens))
+
+    eng._forward = forward
+    monkeypatch.setattr(paged.ops, "sample_tokens", sample)
+    return eng
+
+
+def test_a_request_without_a_token_ends_alone(engine):
+    """sample_tokens gives -1 for a row of no finite logit: that request ends
+    with an error and gives its pages back; the others go on."""
+    ids = [engine.submit(torch.tensor([3, 4, 5]), 4) for _ in range(3)]
+    engine.script = [[7, 8, 9], [10, -1, 11]]
+    out = engine.run()
+    assert out == {ids[0]: [7, 10, 1, 1], ids[1]: [8], ids[2]: [9, 11, 1, 1]}
+    assert engine.finished[ids[1]].error and engine.pool.free == 20
+    assert engine.finished[ids[0]].error is None and engine.finished[ids[2]].error is None
+    engine.script = [[-1]]
+    first = engine.submit(torch.tensor([3]), 2)
+    assert engine.run()[first] == [] and engine.finished[first].error

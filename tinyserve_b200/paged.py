@@ -66,6 +66,7 @@ class PagedRequest:
     logits: list[torch.Tensor] = field(default_factory=list)  # per emitted token, when kept
     pages: list[int] = field(default_factory=list)
     held: int = 0  # positions in the cache
+    error: str | None = None  # why the request ended early
 
     @property
     def done(self) -> bool:
@@ -191,17 +192,16 @@ class PagedServingEngine:
         for r, ids in batch:
             r.held += len(ids)
         due = [i for i, (r, _) in enumerate(batch) if r.held >= len(r.prompt)]
-        if due:
-            self._emit([batch[i][0] for i in due], last[due] if len(due) < len(batch) else last)
+        emitted = self._emit([batch[i][0] for i in due], last[due] if len(due) < len(batch) else last) if due else 0
         for r in [r for r in self.running if r.done]:
             self.running.remove(r)
             self.pool.give_back(r.pages)
             r.pages = []
             self.finished[r.request_id] = r
-        return len(due)
+        return emitted
 
     @torch.no_grad()
-    def _emit(self, requests: list[PagedRequest], last: torch.Tensor) -> None:
+    def _emit(self, requests: list[PagedRequest], last: torch.Tensor) -> int:
         logits = F.linear(last, self.dec.lm_head)
         noise = settings = None
         if any(r.temperature > 0 for r in requests):
@@ -213,17 +213,26 @@ class PagedServingEngine:
                             top_p=torch.tensor([r.top_p for r in requests], device=dev),
                             min_p=torch.tensor([r.min_p for r in requests], device=dev))
         tokens, logprobs = ops.sample_tokens(logits, noise, **(settings or {}))
+        emitted = 0
         for i, (r, t, lp) in enumerate(zip(requests, tokens.tolist(), logprobs.tolist())):
+            if t < 0:
+                # nothing to draw from, and nothing to feed: the others of the batch go on without it
+                r.error = "no token: every logit is NaN or -infinity"
+                r.max_new_tokens = len(r.generated)
+                continue
+            emitted += 1
             r.generated.append(t)
             r.logprobs.append(lp)
             if self.keep_logits:
                 r.logits.append(logits[i].float().cpu())
             if self.eos is not None and t == self.eos:
                 r.max_new_tokens = len(r.generated)
+        return emitted
 
     def run(self) -> dict[int, list[int]]:
         """Serve until every submitted request has finished; returns
-        {request id: generated token ids}."""
+        {request id: generated token ids}.  A request that could not go on
+        ends with what it has; ``finished[id].error`` says why."""
         while self.waiting or self.running:
             self.step()
         return {i: r.generated for i, r in sorted(self.finished.items())}
