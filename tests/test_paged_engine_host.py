@@ -53,3 +53,16 @@ def test_a_request_without_a_token_ends_alone(engine):
     engine.script = [[-1]]
     first = engine.submit(torch.tensor([3]), 2)
     assert engine.run()[first] == [] and engine.finished[first].error
+
+
+def test_submit_refuses_what_a_step_could_not_take(engine):
+    """Ids that are no token would index past the embedding, a top_k past 32
+    bits would fail the whole batch's step."""
+    for bad in (dict(prompt=torch.tensor([3, VOCAB])), dict(prompt=torch.tensor([-1])), dict(top_k=2 ** 31),
+                dict(top_k=-2 ** 31 - 1), dict(top_k=1.5), dict(temperature="warm"), dict(top_p=None)):
+        a = dict(prompt=torch.tensor([3, 4]), max_new_tokens=2) | bad
+        with pytest.raises((ValueError, TypeError)):
+            engine.submit(a.pop("prompt"), a.pop("max_new_tokens"), **a)
+    assert not engine.waiting
+    rid = engine.submit(torch.tensor([0, VOCAB - 1]), 2, temperature=1, top_k=2 ** 31 - 1, top_p=0.5, min_p=0)
+    assert engine.run()[rid] == [1, 1]

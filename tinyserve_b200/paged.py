@@ -14,6 +14,7 @@ go through the LM head to ``ops.sample_tokens``.
 from __future__ import annotations
 
 import itertools
+import operator
 from dataclasses import dataclass, field
 
 import torch
@@ -115,6 +116,13 @@ class PagedServingEngine:
         ids = prompt.reshape(-1).tolist()
         if not ids:
             raise ValueError("empty prompt")
+        vocab = self.dec.embed.shape[0]
+        if min(ids) < 0 or max(ids) >= vocab:
+            raise ValueError(f"prompt ids must be tokens, 0 to {vocab - 1}")
+        temperature, top_p, min_p = float(temperature), float(top_p), float(min_p)
+        top_k = operator.index(top_k)
+        if not -2 ** 31 <= top_k < 2 ** 31:
+            raise ValueError("top_k must fit 32 bits")
         if max_new_tokens < 1:
             raise ValueError("max_new_tokens must be positive")
         if len(ids) + max_new_tokens > self.max_seq:
