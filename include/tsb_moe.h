@@ -390,7 +390,8 @@ typedef struct {
 /* Workspace of the two paged entry points, 256-byte aligned, its first
  * TSB_PAGED_ZEROED bytes zero-initialised once; one workspace serves successive
  * calls on a stream (any batch).  Graphs that may run at the same time need one
- * each.  tsb_read_device_error(workspace, ...) reads its error word. */
+ * each.  tsb_read_device_error(workspace, ...) reads its error word; after a
+ * non-zero one zero those bytes again. */
 #define TSB_PAGED_ZEROED 65536
 size_t tsb_paged_workspace(int32_t head_dim);
 

@@ -24,6 +24,7 @@ def engine(monkeypatch):
     eng.eos, eng.keep_logits = None, False
     eng._ids, eng._rng = itertools.count(), torch.Generator()
     eng.waiting, eng.running, eng.finished = [], [], {}
+    eng._scratch = [torch.zeros(64, dtype=torch.uint8) for _ in range(2)]
     eng.fed, eng.script = [], []
 
     def forward(batch):
@@ -66,3 +67,16 @@ def test_submit_refuses_what_a_step_could_not_take(engine):
     assert not engine.waiting
     rid = engine.submit(torch.tensor([0, VOCAB - 1]), 2, temperature=1, top_k=2 ** 31 - 1, top_p=0.5, min_p=0)
     assert engine.run()[rid] == [1, 1]
+
+
+def test_device_errors_end_what_is_under_way(engine):
+    """An error word that a kernel set: no token of that step is handed out, the
+    requests under way end with an error, those that wait are served after."""
+    ids = [engine.submit(torch.tensor([3, 4, 5]), 3) for _ in range(5)]  # one more than max_batch
+    engine.step()
+    engine._scratch[1].fill_(1)
+    assert engine.step() == 0
+    for i in ids[:4]:
+        assert engine.finished[i].generated == [1] and "device error" in engine.finished[i].error
+    assert engine.pool.free == 20 and not any(t.any() for t in engine._scratch)
+    assert engine.run()[ids[4]] == [1, 1, 1] and engine.finished[ids[4]].error is None

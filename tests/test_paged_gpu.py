@@ -556,3 +556,16 @@ def test_windows_and_first_tokens_of_any_size(ops, window, keep, held):
         b = R.Batch(*lens, 8, 1, 64, 16, BF, held, seed=7)
         kw = dict(window=window, keep_first=keep)
         check(attend(ops, b, **kw), b, **kw)
+
+
+def test_scratch_is_sound_again_after_an_error_is_read(ops):
+    """A call that gave up half way leaves its counts of finished parts behind;
+    reading its error word clears them with it."""
+    ws = ops.paged_workspace(torch.device("cuda"), 64)
+    ws[:1 << 16].view(torch.int32)[64:4096] = 1000  # every counter
+    ws[:4].view(torch.int32)[0] = 1
+    assert ops.paged_device_error(ws) == 1
+    assert ops.paged_device_error(ws) == 0
+    for lens in (([1, 2], [9000, 5000]), ([40], [6001])):  # divided and joined
+        b = R.Batch(*lens, 8, 1, 64, 64, BF, BF, seed=3)
+        check(attend(ops, b, workspace=ws), b)

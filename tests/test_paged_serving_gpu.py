@@ -181,3 +181,17 @@ def test_steps_of_any_size_take_no_more_memory(lm):
     serve(40)
     few = serve(16)
     assert all(serve(n) <= few + (1 << 20) for n in [*range(39, 16, -1), *range(15, 0, -1)])
+
+
+def test_device_errors_are_read(lm):
+    """A page that is none in a request's list: the requests of that step end with an error, later ones are served."""
+    eng = engine(lm)
+    first = eng.submit(prompts((20,))[0], 4)
+    eng.step()
+    eng.running[0].pages[0] = 10 ** 6
+    eng.step()
+    assert "device error" in eng.finished[first].error and len(eng.finished[first].generated) == 1
+    eng.pool._free = list(range(40))
+    again = eng.submit(prompts((20,))[0], 4)
+    eng.run()
+    assert eng.finished[again].error is None and len(eng.finished[again].generated) == 4

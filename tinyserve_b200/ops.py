@@ -122,11 +122,13 @@ def paged_device_error(workspace: torch.Tensor | None = None, device: torch.devi
     workspace the paged operators keep for ``device`` (of a stream's graphs with
     scratch of their own, the last captured one's): 0 when the batches were
     consistent, 2 when one named a page outside the pool or a length beyond
-    its table.  Synchronises."""
+    its table, 1 when a wait inside a kernel gave up.  After an error the
+    workspace is made sound again.  Synchronises."""
     if workspace is None:
-        device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+        device = torch.device("cuda" if device is None else device)
+        index = torch.cuda.current_device() if device.index is None else device.index
         kept = list(_paged_ws.items()) + [(key, ws) for key, (_, ws) in _captured_ws.items()]
-        held = [ws for key, ws in kept if key[0] == (device.index or 0)]
+        held = [ws for key, ws in kept if key[0] == index]
     else:
         held = [workspace]
     code = 0
@@ -134,6 +136,9 @@ def paged_device_error(workspace: torch.Tensor | None = None, device: torch.devi
         torch.cuda.synchronize(ws.device)
         c = ctypes.c_int32()
         _lib.check(_lib.lib().tsb_read_device_error(ws.data_ptr(), ctypes.byref(c), _stream(ws.device)))
+        if c.value:
+            ws[:_PAGED_ZEROED].zero_()  # a call that gave up leaves counts of finished parts
+            torch.cuda.synchronize(ws.device)
         code = code or c.value
     return code
 

@@ -102,6 +102,10 @@ class PagedServingEngine:
             moe = lay["moe"]
             need[moe.dense] = max([need[moe.dense]] + [moe.workspace_bytes(t) for t in range(ONE_BY_ONE + 1, chunk_tokens + 1)])
         self._expert_ws = {k: torch.zeros(n, dtype=torch.uint8, device=d.device) for k, n in need.items()}
+        self._ws = ops.paged_workspace(d.device, d.D)
+        # every scratch of a step, each with its error word in front
+        self._scratch = [self._ws] + [t for t in self._expert_ws.values() if t.numel()]
+        self._scratch += [lay["moe"].workspace(1) for lay in d.layers]
         self.eos = eos_token_id
         self.keep_logits = keep_logits
         self._ids = itertools.count()
@@ -180,9 +184,11 @@ class PagedServingEngine:
         d._norm(x, None, d.layers[0]["ln1"], h)
         for li, lay in enumerate(d.layers):
             qkv = F.linear(h, lay["wqkv"], lay["bqkv"])
-            q = ops.paged_kv_store(qkv, self.cos, self.sin, pool.k[li], pool.v[li], pages, cu, kv, n_q_heads=d.nq)
+            q = ops.paged_kv_store(qkv, self.cos, self.sin, pool.k[li], pool.v[li], pages, cu, kv, n_q_heads=d.nq,
+                                   workspace=self._ws)
             a = ops.paged_attention(q, pool.k[li], pool.v[li], pages, cu, kv, max_q, scale=d.scale,
-                                    window=d.window if d.sliding[li] else 0, sinks=lay["sinks"])
+                                    window=d.window if d.sliding[li] else 0, sinks=lay["sinks"],
+                                    workspace=self._ws)
             d._norm(x, F.linear(a.view(a.shape[0], -1), lay["wo"], lay["bo"]), lay["ln2"], h)
             moe = lay["moe"]
             y, _, _ = moe.decode(h, out_dtype=torch.float32, workspace=self._expert_ws[moe.dense])
@@ -208,6 +214,15 @@ class PagedServingEngine:
             self.finished[r.request_id] = r
         return emitted
 
+    def _device_error(self) -> int:
+        """The first error a kernel has reported since the last call, 0 for none; what it left behind is cleared."""
+        codes = torch.cat([t[:4].view(torch.int32) for t in self._scratch]).tolist()
+        code = next((c for c in codes if c), 0)
+        if code:
+            for t in self._scratch:
+                t.zero_()
+        return code
+
     @torch.no_grad()
     def _emit(self, requests: list[PagedRequest], last: torch.Tensor) -> int:
         logits = F.linear(last, self.dec.lm_head)
@@ -221,6 +236,13 @@ class PagedServingEngine:
                             top_p=torch.tensor([r.top_p for r in requests], device=dev),
                             min_p=torch.tensor([r.min_p for r in requests], device=dev))
         tokens, logprobs = ops.sample_tokens(logits, noise, **(settings or {}))
+        code = self._device_error()
+        if code:
+            # of this step or one before that emitted nothing: no cache under way is to be trusted
+            for r in self.running:
+                r.error = f"device error {code}"
+                r.max_new_tokens = len(r.generated)
+            return 0
         emitted = 0
         for i, (r, t, lp) in enumerate(zip(requests, tokens.tolist(), logprobs.tolist())):
             if t < 0:
