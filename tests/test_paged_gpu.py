@@ -569,3 +569,29 @@ def test_scratch_is_sound_again_after_an_error_is_read(ops):
     for lens in (([1, 2], [9000, 5000]), ([40], [6001])):  # divided and joined
         b = R.Batch(*lens, 8, 1, 64, 64, BF, BF, seed=3)
         check(attend(ops, b, workspace=ws), b)
+
+
+def test_arguments_elsewhere_are_refused(ops):
+    """Scratch, tables and sinks that no kernel on this GPU could read, and
+    scratch whose bytes are not what its numel says."""
+    b = R.Batch([1], [5], 8, 2, 64, 16, BF, BF)
+    n = ops.paged_workspace(torch.device("cuda"), 64).numel()
+    t = torch.rand(8, 32, device="cuda")
+    qkv = torch.zeros(1, 12 * 64, dtype=BF, device="cuda")
+    for ws in (torch.zeros(n, dtype=torch.uint8), torch.zeros(n, dtype=torch.uint8).pin_memory(),
+               torch.zeros(n // 4, dtype=torch.float32, device="cuda"),
+               torch.zeros(2 * n, dtype=torch.uint8, device="cuda")[::2],
+               torch.zeros(1, dtype=torch.uint8, device="cuda").expand(n)):
+        with pytest.raises((RuntimeError, ValueError)):
+            attend(ops, b, workspace=ws)
+        with pytest.raises((RuntimeError, ValueError)):
+            ops.paged_kv_store(qkv, t, t, b.k, b.v, b.table, b.cu, b.kv, n_q_heads=8, workspace=ws)
+    for name in ("k", "v", "table", "cu", "kv", "sinks", "q"):
+        c = R.Batch([1], [5], 8, 2, 64, 16, BF, BF)
+        setattr(c, name, getattr(c, name).cpu())
+        with pytest.raises((RuntimeError, ValueError)):
+            attend(ops, c)
+    for kw in (dict(cos=t.cpu()), dict(sin=t.cpu()), dict(q_out=torch.empty(1, 8, 64, dtype=BF))):
+        a = dict(cos=t, sin=t) | kw
+        with pytest.raises((RuntimeError, ValueError)):
+            ops.paged_kv_store(qkv, a.pop("cos"), a.pop("sin"), b.k, b.v, b.table, b.cu, b.kv, n_q_heads=8, **a)

@@ -30,6 +30,17 @@ def _require_cuda(*ts: torch.Tensor | None) -> None:
             raise RuntimeError("tinyserve_b200 kernels need CUDA tensors")
 
 
+def _require_one_device(first: torch.Tensor, *others: torch.Tensor | None) -> None:
+    device = first.get_device()
+    if device >= 0:
+        for t in others:
+            if t is not None and t.get_device() != device:
+                break
+        else:
+            return
+    raise RuntimeError("tinyserve_b200 kernels need CUDA tensors, all on one device")
+
+
 def dequant(fmt: int, w: torch.Tensor, scales: torch.Tensor | None, rows: int, cols: int,
             dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """Bit-exact dequantisation (same values as ``dequant_tensor`` /
@@ -144,12 +155,12 @@ def paged_device_error(workspace: torch.Tensor | None = None, device: torch.devi
 
 
 def _paged_call(rows: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
-                cu_q: torch.Tensor, kv_lens: torch.Tensor, max_q: int):
+                cu_q: torch.Tensor, kv_lens: torch.Tensor, max_q: int, workspace: torch.Tensor | None):
     """The C structs of a paged call (kept alive by the caller), after the
     checks that need the tensors themselves."""
-    if not (rows.is_cuda and k_cache.is_cuda and v_cache.is_cuda and page_table.is_cuda and cu_q.is_cuda
-            and kv_lens.is_cuda):
-        raise RuntimeError("tinyserve_b200 kernels need CUDA tensors")
+    _require_one_device(rows, k_cache, v_cache, page_table, cu_q, kv_lens, workspace)
+    if workspace is not None and (workspace.dtype != torch.uint8 or not workspace.is_contiguous()):
+        raise ValueError("workspace must be contiguous uint8")
     dtype, held = rows.dtype, k_cache.dtype
     if dtype != torch.bfloat16 and dtype != torch.float16:
         raise TypeError("tokens must be bfloat16 or float16")
@@ -189,13 +200,13 @@ def paged_kv_store(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_ca
     kv_lens     int32 [B]: positions held once the new tokens are in; those are its last ones
     """
     n, d = qkv.shape[0], k_cache.shape[-1]
-    cache, batch = _paged_call(qkv, k_cache, v_cache, page_table, cu_q, kv_lens, n)
+    cache, batch = _paged_call(qkv, k_cache, v_cache, page_table, cu_q, kv_lens, n, workspace)
     if qkv.dim() != 2 or qkv.shape[1] != (n_q_heads + 2 * cache.n_kv_heads) * d or (n and qkv.stride(1) != 1):
         raise ValueError("qkv must be [tokens, (n_q_heads + 2 kv_heads) * head_dim] with contiguous rows")
     if (cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != sin.dtype or cos.shape[1] * 2 != d
             or cos.dtype not in _DT or not cos.is_contiguous() or not sin.is_contiguous()):
         raise ValueError("cos and sin must be contiguous [positions, head_dim / 2] of fp32, bf16 or f16")
-    _require_cuda(cos, sin, q_out)
+    _require_one_device(qkv, cos, sin, q_out)
     if q_out is None:
         q_out = torch.empty(n, n_q_heads, d, dtype=qkv.dtype, device=qkv.device)
     elif q_out.shape != (n, n_q_heads, d) or q_out.dtype != qkv.dtype or not q_out.is_contiguous():
@@ -223,16 +234,16 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     sinks       fp32 [n_q_heads]: a logit per head that joins the softmax denominator only
     The other arguments are paged_kv_store's.  A token that sees nothing gives zeros.
     """
-    cache, batch = _paged_call(q, k_cache, v_cache, page_table, cu_q, kv_lens, max_q)
+    cache, batch = _paged_call(q, k_cache, v_cache, page_table, cu_q, kv_lens, max_q, workspace)
     n, d = q.shape[0], cache.head_dim
     if q.dim() != 3 or q.shape[2] != d or (n and q.stride(2) != 1):
         raise ValueError("q must be [tokens, n_q_heads, head_dim] with a contiguous last dimension")
     if sinks is not None and (sinks.dtype != torch.float32 or sinks.shape != (q.shape[1],) or not sinks.is_contiguous()
-                              or not sinks.is_cuda):
+                              or sinks.get_device() != q.get_device()):
         raise ValueError("sinks must be fp32 [n_q_heads] on the GPU")
     if out is None:
         out = torch.empty(n, q.shape[1], d, dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous() or not out.is_cuda:
+    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous() or out.device != q.device:
         raise ValueError("out must be contiguous, like q")
     stream = _stream_of(q)
     ws = _paged_workspace(q.device, d, stream) if workspace is None else workspace
@@ -258,7 +269,7 @@ def sample_tokens(logits: torch.Tensor, noise: torch.Tensor | None = None, *,
                  the best token; the best token is always kept.
     logprobs     of the drawn tokens under the row's softmax at its temperature, before the filters
     """
-    _require_cuda(logits, noise, temperature, top_k, top_p, min_p)
+    _require_one_device(logits, noise, temperature, top_k, top_p, min_p)
     if logits.dim() != 2 or logits.dtype not in _DT:
         raise ValueError("logits must be [rows, vocabulary] of fp32, bf16 or f16")
     rows, vocab = logits.shape
