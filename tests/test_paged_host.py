@@ -86,3 +86,24 @@ def test_sample_refusals():
                      (dict(x=None), 1), (dict(tokens=None), 1)):
         assert sample(**kw) == code, kw
     assert sample(rows=0) == 0
+
+
+def test_pointers_off_their_type_are_refused():
+    """An element that crosses its own alignment would fault on the device."""
+    L = _lib.lib()
+    for dt, off in ((_lib.DT_F32, 2), (_lib.DT_BF16, 1), (_lib.DT_F16, 1)):
+        assert L.tsb_sample(P + off, dt, 2, 8, 8, P, 8, None, None, None, None, P, None, None) == _lib.TSB_ERR_INVALID
+        assert "aligned" in _lib.last_error()
+    for at in range(5, 13):
+        if at == 6:  # noise_stride
+            continue
+        a = [P, 0, 2, 8, 8, P, 8, P, P, P, P, P, P, None]
+        a[at] = P + (4 if at == 11 else 2)
+        assert L.tsb_sample(*a) == _lib.TSB_ERR_INVALID, at
+        assert "aligned" in _lib.last_error()
+    for name in ("page_table", "cu_q", "kv_lens"):
+        assert attention(b=batch(**{name: P + 2})) == _lib.TSB_ERR_INVALID
+        assert "aligned" in _lib.last_error()
+    rc = L.tsb_paged_attention(ctypes.byref(cache()), ctypes.byref(batch()), P, 512, 64, 8, 0, 0, P + 2, 0.125, P, P,
+                               1 << 30, None)
+    assert rc == _lib.TSB_ERR_INVALID and "aligned" in _lib.last_error()

@@ -188,6 +188,9 @@ int paged_args(const TsbPagedCache* c, const TsbPagedBatch* b, int n_q_heads, vo
   if (b->n_tokens > 0 && b->n_seqs > 0 &&
       (!c->k_cache || !c->v_cache || !b->cu_q || !b->kv_lens || (b->table_width > 0 && !b->page_table)))
     return fail(TSB_ERR_INVALID, "null pointer");
+  if ((reinterpret_cast<uintptr_t>(b->page_table) | reinterpret_cast<uintptr_t>(b->cu_q) |
+       reinterpret_cast<uintptr_t>(b->kv_lens)) & 3)
+    return fail(TSB_ERR_INVALID, "page_table, cu_q and kv_lens must be 4-byte aligned");
   if (reinterpret_cast<uintptr_t>(ws) & 255) return fail(TSB_ERR_INVALID, "workspace must be 256-byte aligned");
   if (ws_bytes < tsb_paged_workspace(c->head_dim)) return fail(TSB_ERR_WORKSPACE, "workspace too small");
   a.kc = static_cast<const uint8_t*>(c->k_cache);
@@ -293,6 +296,7 @@ int tsb_paged_attention(const TsbPagedCache* cache, const TsbPagedBatch* batch, 
     return fail(TSB_ERR_INVALID, "q strides must be multiples of 8 elements");
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15)
     return fail(TSB_ERR_INVALID, "q and out must be 16-byte aligned");
+  if (reinterpret_cast<uintptr_t>(sinks) & 3) return fail(TSB_ERR_INVALID, "sinks must be 4-byte aligned");
   c.q = static_cast<const uint16_t*>(q);
   c.out = static_cast<uint16_t*>(out);
   c.q_token_stride = q_token_stride;

@@ -750,6 +750,10 @@ extern "C" int tsb_sample(const void* logits, int32_t dtype, int32_t rows, int32
   if (row_stride < vocab || (noise && noise_stride < vocab)) return set_error(TSB_ERR_INVALID, "rows must not overlap");
   if (rows == 0) return TSB_OK;
   if (!logits || !tokens) return set_error(TSB_ERR_INVALID, "null pointer");
+  const auto off = [](const void* p, uintptr_t size) { return reinterpret_cast<uintptr_t>(p) % size != 0; };
+  if (off(logits, dtype == TSB_DT_F32 ? 4 : 2) || off(noise, 4) || off(temperature, 4) || off(top_k, 4) ||
+      off(top_p, 4) || off(min_p, 4) || off(tokens, 8) || off(logprobs, 4))
+    return set_error(TSB_ERR_INVALID, "pointers must be aligned to their type");
   SampleArgs a{logits, noise,  temperature, top_k,        top_p, min_p,
                tokens, logprobs, row_stride,  noise_stride, vocab, 0, 1};
   while ((1 << a.index_bits) < vocab) ++a.index_bits;
