@@ -595,3 +595,32 @@ def test_arguments_elsewhere_are_refused(ops):
         a = dict(cos=t, sin=t) | kw
         with pytest.raises((RuntimeError, ValueError)):
             ops.paged_kv_store(qkv, a.pop("cos"), a.pop("sin"), b.k, b.v, b.table, b.cu, b.kv, n_q_heads=8, **a)
+
+
+@pytest.mark.parametrize("q_len", [1, 3, 0])
+def test_more_sequences_than_a_launch_takes(ops, q_len):
+    """Over 512 sequences, which the kernels take in several launches: all of one
+    length, or (0) of every length up to 20."""
+    n = 700
+    q_lens = [q_len or i % 21 for i in range(n)]
+    b = R.Batch(q_lens, [q + (13 * i) % 90 for i, q in enumerate(q_lens)], 8, 1, 64, 16, BF, BF, seed=q_len)
+    check(attend(ops, b), b)
+
+
+def test_tables_of_the_widest_kind(ops):
+    """Nearly 2^30 positions a sequence in the table (of which few are used): the
+    launches take fewer sequences, so that their steps can be counted."""
+    page = 1 << 20
+    narrow = R.Batch([1] * 70 + [3] * 8 + [40], [60 + i for i in range(79)], 8, 1, 128, 128, BF, E4, seed=2)
+    k = torch.zeros(narrow.k.shape[0] * 128 // page + 1, 1, page, 128, dtype=E4, device="cuda")
+    v = torch.zeros_like(k)
+    table = torch.zeros(79, (1 << 30) // page - 1, dtype=torch.int32, device="cuda")
+    got = torch.empty_like(narrow.q)
+    for i in range(79):  # one at a time: each has its positions at the start of page 0
+        for pool, small in ((k, narrow.k), (v, narrow.v)):
+            pool[0, :, :128] = small[int(narrow.table[i, 0])]
+            pool[0, :, 128:256] = small[int(narrow.table[i, 1])] if narrow.kv_lens[i] > 128 else 0
+        out = ops.paged_attention(narrow.q, k, v, table, narrow.cu, narrow.kv, 40, sinks=narrow.sinks)
+        rows = slice(int(narrow.cu[i]), int(narrow.cu[i + 1]))
+        got[rows] = out[rows]
+    check(got, narrow)

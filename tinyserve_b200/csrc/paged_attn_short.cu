@@ -631,14 +631,16 @@ int launch_paged_short(const TsbPagedCache& cache, const AttnCall& call, cudaStr
     constexpr int DT = decltype(dt)::value, D = decltype(d)::value;
     constexpr bool FP8 = decltype(fp8)::value;
     ShortArgs a{call};
-    for (int b0 = 0; b0 < call.p.n_seqs && e == cudaSuccess; b0 += kMaxSeqs) {
+    // a launch's sequences: their steps are summed in 32 bits
+    const int steps = call.p.max_pos / step_of<D>() + 3 + kItemCost;
+    const int seqs = min(kMaxSeqs, INT32_MAX / steps);
+    for (int b0 = 0; b0 < call.p.n_seqs && e == cudaSuccess; b0 += seqs) {
       a.c.p.table = call.p.table + (int64_t)b0 * call.p.table_stride;
       a.c.p.cu_q = call.p.cu_q + b0;
       a.c.p.kv_lens = call.p.kv_lens + b0;
-      a.c.p.n_seqs = min(kMaxSeqs, call.p.n_seqs - b0);
+      a.c.p.n_seqs = min(seqs, call.p.n_seqs - b0);
       // no more CTAs than pieces of the least size in the longest tables
-      const int64_t most = (int64_t)a.c.p.n_seqs * call.p.nkv *
-                           ((call.p.max_pos / step_of<D>() + 3 + kItemCost) / kMinPiece + 1);
+      const int64_t most = (int64_t)a.c.p.n_seqs * call.p.nkv * (steps / kMinPiece + 1);
       auto kern = paged_attn_short<DT, D, FP8>;
       using Rg = Ring<D, FP8>;
       constexpr int smem = Rg::kBytes > (int)sizeof(Sums<D>) ? Rg::kBytes : (int)sizeof(Sums<D>);
