@@ -107,3 +107,17 @@ def test_pointers_off_their_type_are_refused():
     rc = L.tsb_paged_attention(ctypes.byref(cache()), ctypes.byref(batch()), P, 512, 64, 8, 0, 0, P + 2, 0.125, P, P,
                                1 << 30, None)
     assert rc == _lib.TSB_ERR_INVALID and "aligned" in _lib.last_error()
+
+
+def test_store_refuses_pools_whose_rows_overlap():
+    """An expanded pool has one place for several heads' (rows', pages') values; reading one is fine."""
+    L = _lib.lib()
+
+    def store(c):
+        return L.tsb_paged_kv_store(ctypes.byref(c), ctypes.byref(batch()), P, 1280, 8, P, P, _lib.DT_F32, 64, P, P,
+                                    1 << 30, None)
+
+    ok = dict(n_kv_heads=2, page_stride=2 * 16 * 64, head_stride=16 * 64, row_stride=64)
+    for kw in (dict(head_stride=0), dict(row_stride=0), dict(page_stride=0), dict(row_stride=32)):
+        assert store(cache(**ok | kw)) == _lib.TSB_ERR_INVALID, kw
+        assert "overlap" in _lib.last_error()

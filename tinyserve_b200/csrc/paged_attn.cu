@@ -256,6 +256,10 @@ int tsb_paged_kv_store(const TsbPagedCache* cache, const TsbPagedBatch* batch, c
   if (!qkv || !cos || !sin || !q_out) return fail(TSB_ERR_INVALID, "null pointer");
   if (qkv_stride < (int64_t)(n_q_heads + 2 * cache->n_kv_heads) * cache->head_dim || qkv_stride % 8)
     return fail(TSB_ERR_INVALID, "qkv rows must not overlap and be a multiple of 8 elements apart");
+  const auto overlaps = [&](int n, int64_t stride) { return n > 1 && stride < cache->head_dim; };
+  if (overlaps(cache->n_kv_heads, cache->head_stride) || overlaps(cache->page_size, cache->row_stride) ||
+      overlaps(cache->num_pages, cache->page_stride))
+    return fail(TSB_ERR_INVALID, "rows of the caches must not overlap");
   if ((reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(cos) | reinterpret_cast<uintptr_t>(sin) |
        reinterpret_cast<uintptr_t>(q_out)) & 15)
     return fail(TSB_ERR_INVALID, "qkv, cos, sin and q_out must be 16-byte aligned");
