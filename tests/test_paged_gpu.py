@@ -624,3 +624,14 @@ def test_tables_of_the_widest_kind(ops):
         rows = slice(int(narrow.cu[i]), int(narrow.cu[i + 1]))
         got[rows] = out[rows]
     check(got, narrow)
+
+
+@pytest.mark.parametrize("dtype,held,page", [(BF, "same", 16), (BF, "same", 100), (F16, "same", 24), (BF, "e4m3", 16),
+                                             (F16, "e4m3", 1)])
+@pytest.mark.parametrize("window,keep", [(1, 3), (37, 4), (128, 140), (1000, 5)])
+def test_windows_of_wide_heads(ops, window, keep, dtype, held, page):
+    """Windows and first tokens at D = 128, by every way that pages are read."""
+    for lens in (RAGGED, ([1, 1, 3, 1], [900, 129, 500, 20]), ([200, 70], [640, 1500])):
+        b = R.Batch(*lens, 8, 2, 128, page, dtype, E4 if held == "e4m3" else dtype, seed=window + keep)
+        kw = dict(window=window, keep_first=keep)
+        check(attend(ops, b, **kw), b, **kw)
