@@ -268,16 +268,6 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows(const SampleArgs a) {
     if (v == top) return 0.f;
     return top == INFINITY || v == -INFINITY ? -INFINITY : fmaxf(v - top, -FLT_MAX) * inv;
   };
-  // A token's weight, from one formula wherever masses are added: a limit that lies
-  // in a bin lies in one of its parts too.
-  const bool tame = top < INFINITY && inv > 1e-30f && inv < 1e30f;  // no 0 * infinity, no infinity - infinity
-  const float inv_log2e = inv * 1.4426950408889634f;
-  const auto weight_at = [&](float d) {  // of a distance, in a tame row
-    float w;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(d * inv_log2e));
-    return w;
-  };
-  const auto weight = [&](float v) { return tame ? weight_at(fmaxf(v - top, -FLT_MAX)) : expf(scaled(v)); };
   const auto mass_of = [&](float w) { return __float2uint_rn(w * 2147483648.f); };  // in units of 2^-31
   const auto bin_of = [&](float v) {  // distance from the maximum, monotone in the logit
     const float d = v == top ? 0.f : top - v;
@@ -478,14 +468,16 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows(const SampleArgs a) {
       part = s;
     };
     const bool free_race = !filtered && !by_min && !greedy;
-    if (tame) {
+    if (top < INFINITY && inv > 1e-30f && inv < 1e30f) {  // no 0 * infinity, no infinity - infinity
+      const float c = inv * 1.4426950408889634f;
       each([&](int i, const float(&v)[PER]) {
         float d[PER], z[PER];
         if (free_race) noise_of(i, v, z);
 #pragma unroll
         for (int e = 0; e < PER; ++e) {
           d[e] = fmaxf(v[e] - top, -FLT_MAX);
-          const float w = weight_at(d[e]);
+          float w;
+          asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(d[e] * c));
           add(w);
           if (mass_first && v[e] > -INFINITY) put(bin_of(v[e]), w);
         }
@@ -527,7 +519,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows(const SampleArgs a) {
       uint32_t at;
       asm volatile("atom.shared::cluster.add.u32 %0, [%1], 1;" : "=r"(at) : "r"(counter) : "memory");
       if (at < kList) {
-        const uint32_t m = by_p ? mass_of(weight(v)) : 0u;
+        const uint32_t m = by_p ? mass_of(expf(scaled(v))) : 0u;
         asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(keys + 8 * at), "l"(key) : "memory");
         asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(masses + 4 * at), "r"(m) : "memory");
       }
@@ -555,7 +547,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows(const SampleArgs a) {
       if (!ready) {
         if (dirty) clear();
         visit([&](int i, float v) {
-          if (counts(i, v)) put(bin_of(v), by_p ? weight(v) : 0.f);
+          if (counts(i, v)) put(bin_of(v), by_p ? expf(scaled(v)) : 0.f);
         });
       }
       ready = false;
@@ -605,14 +597,20 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows(const SampleArgs a) {
         shift = max(0, 64 - __clzll((long long)(key_hi - key_lo)) - 10);
         clear();
         visit([&](int i, float v) {
-          if (in_range(i, v)) put((int)((key_hi - key_of(v, i)) >> shift), by_p ? weight(v) : 0.f);
+          if (in_range(i, v)) put((int)((key_hi - key_of(v, i)) >> shift), by_p ? expf(scaled(v)) : 0.f);
         });
         combine();
         scan(count, bn, bm, want);
       }
       const int bin = sh.bin;
-      if (bin < 0) {  // fewer tokens than k; or rounding leaves the limit past the last (of the whole row)
+      if (bin < 0) {
+        // Fewer tokens than k; or rounding leaves the limit past the last token: of
+        // the row, or of the bin that was divided, whose masses come from another
+        // exponential the second time.  That bin is kept to its end.
         if (count) todo_k = false;
+        if (level > 0) threshold = more(threshold, key_lo);
+        if (cap < INFINITY) listed = false;
+        cap = INFINITY;
         continue;
       }
       const uint32_t bn = sh.before_count;
