@@ -34,10 +34,11 @@
 // copies its 16-byte pieces ahead into shared memory with a ring of
 // asynchronous copies; held in registers they were waited for when the ring
 // moved on, and loops unrolled over several loads were bound by their own
-// first fetch.  Measured (201088 tokens): one fp32 row with top-p 35 us; 32 fp32 rows
-// without filters 30 us (1.7 TB/s of logits and noise); 64 bf16 rows 33 us with
-// min-p, 41 us with top-k, 112 us with top-p, whose warm rows keep more tokens
-// than the lists hold and take two more passes.
+// first fetch.  Measured (201088 tokens): one fp32 row with top-p 34 us; 32 fp32 rows
+// without filters 28 us (1.8 TB/s of logits and noise); 64 bf16 rows 27 us greedy,
+// 45 us without filters, 34 us with min-p, 41 us with top-k, with top-p of 0.9 69 us at
+// temperature 0.7 and 118 us at 1, where rows keep more tokens than the lists
+// hold and take two more passes.
 #include <cfloat>
 
 #include "tc05.cuh"

@@ -198,6 +198,8 @@ def paged_kv_store(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_ca
     page_table  int32 [B, pages per sequence]
     cu_q        int32 [B + 1]: rows of sequence b are cu_q[b] .. cu_q[b + 1] - 1
     kv_lens     int32 [B]: positions held once the new tokens are in; those are its last ones
+    workspace   scratch of ``paged_workspace`` instead of the stream's own
+    Rows that belong to no sequence are not written (in a new q_out they hold anything).
     """
     n, d = qkv.shape[0], k_cache.shape[-1]
     cache, batch = _paged_call(qkv, k_cache, v_cache, page_table, cu_q, kv_lens, n, workspace)
@@ -232,7 +234,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     max_q       upper bound of the new tokens of any sequence
     window      0: every earlier position; else the last ``window`` positions and the first ``keep_first``
     sinks       fp32 [n_q_heads]: a logit per head that joins the softmax denominator only
-    The other arguments are paged_kv_store's.  A token that sees nothing gives zeros.
+    The other arguments are paged_kv_store's.  A token that sees nothing gives zeros; rows that belong to no sequence
+    are not written (in a new ``out`` they hold anything).
     """
     cache, batch = _paged_call(q, k_cache, v_cache, page_table, cu_q, kv_lens, max_q, workspace)
     n, d = q.shape[0], cache.head_dim
